@@ -203,11 +203,12 @@ def prepare(case, seed):
          'kv_len': torch.tensor(total, dtype=torch.int32, device=DEV),
          'k_scale': None, 'v_scale': None, 'prefix_len': None, 'q_start': None}
     if case['cache'] == 'e4m3':
-        # the largest of normal values, with room, at e4m3's largest
+        # scales near the largest normal value over e4m3's largest; the cast
+        # makes NaN of what is beyond, so clamp
         u = torch.rand(2, kv, generator=g, device=DEV) * 0.4 + 0.8
         s['k_scale'], s['v_scale'] = (u * (6.0 / 448.0)).unbind(0)
-        k = (k / s['k_scale'].view(-1, 1, 1)).to(F8).view(torch.uint8)
-        v = (v / s['v_scale'].view(-1, 1, 1)).to(F8).view(torch.uint8)
+        k = (k / s['k_scale'].view(-1, 1, 1)).clamp_(-448, 448).to(F8).view(torch.uint8)
+        v = (v / s['v_scale'].view(-1, 1, 1)).clamp_(-448, 448).to(F8).view(torch.uint8)
     s['k'], s['v'] = k, v
     if case['prefix']:
         s['prefix_len'] = torch.tensor([min(case['prefix'], t) for t in total],
