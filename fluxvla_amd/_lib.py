@@ -153,6 +153,48 @@ class AttnBwdDesc(ctypes.Structure):
         ('scale', c_f32),
     ]
 
+
+class PagedAppendDesc(ctypes.Structure):
+    """Mirror of ``fvx_paged_append_desc``."""
+    _fields_ = [
+        ('qkv', c_vp), ('ld_qkv', c_i64),
+        ('q_out', c_vp), ('ld_q', c_i64),
+        ('k', c_vp), ('v', c_vp),
+        ('k_scale', c_vp), ('v_scale', c_vp),
+        ('rope', c_vp), ('max_pos', c_i64),
+        ('positions', c_vp),
+        ('page_table', c_vp), ('table_stride', c_i64),
+        ('kv_len', c_vp),
+        ('q_start', c_vp),
+        ('n_rows', c_i64), ('n_seqs', c_i64), ('max_pages', c_i64),
+        ('n_pages', c_i64), ('page_size', c_i64), ('q_heads', c_i64),
+        ('kv_heads', c_i64), ('head_dim', c_i64),
+        ('e4m3', c_i32),
+    ]
+
+
+class PagedAttnDesc(ctypes.Structure):
+    """Mirror of ``fvx_paged_attn_desc``."""
+    _fields_ = [
+        ('q', c_vp), ('ldq', c_i64),
+        ('o', c_vp), ('ldo', c_i64),
+        ('k', c_vp), ('v', c_vp),
+        ('k_scale', c_vp), ('v_scale', c_vp),
+        ('page_table', c_vp), ('table_stride', c_i64),
+        ('kv_len', c_vp),
+        ('q_start', c_vp),
+        ('prefix_len', c_vp),
+        ('n_rows', c_i64), ('n_seqs', c_i64), ('max_pages', c_i64),
+        ('max_q', c_i64),
+        ('n_pages', c_i64), ('page_size', c_i64), ('q_heads', c_i64),
+        ('kv_heads', c_i64), ('head_dim', c_i64),
+        ('window', c_i64),
+        ('scale', c_f32), ('softcap', c_f32),
+        ('e4m3', c_i32),
+        ('workspace', c_vp), ('workspace_bytes', c_i64),
+    ]
+
+
 # name -> (restype, argtypes); the exact set declared by include/fluxvla_amd.h
 SIGNATURES = {
     'fvx_version': (c_i32, []),
@@ -211,6 +253,10 @@ SIGNATURES = {
     'fvx_rtc_vjp_update': (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,
                                    c_vp, c_i64, c_vp, c_vp, c_i64, c_vp,
                                    c_i64, c_i64, c_i64, c_f32, c_f32, c_vp]),
+    # paged key/value cache
+    'fvx_paged_append': (c_i32, [ctypes.POINTER(PagedAppendDesc), c_vp]),
+    'fvx_paged_attention': (c_i32, [ctypes.POINTER(PagedAttnDesc), c_vp]),
+    'fvx_paged_attention_workspace_bytes': (c_i64, [ctypes.POINTER(PagedAttnDesc)]),
 }
 
 ACT_BWD_GEGLU, ACT_BWD_SILU = 0, 1

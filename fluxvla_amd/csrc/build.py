@@ -15,7 +15,8 @@ PKG = os.path.dirname(HERE)
 OUT = os.path.join(PKG, 'libfluxvla_amd.so')
 OBJ_DIR = os.path.join(HERE, '_build')
 SOURCES = ['norm.hip', 'gemm.hip', 'gemm_mid.hip', 'gemm_pp.hip', 'attention.hip',
-           'attention_encoder.hip', 'misc.hip', 'preprocess.hip', 'backward.hip']
+           'attention_encoder.hip', 'misc.hip', 'preprocess.hip', 'backward.hip',
+           'paged_append.hip', 'paged_attention.hip']
 ARCH = 'gfx950'
 
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')

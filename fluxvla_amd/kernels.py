@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import AttnDesc, GemmDesc
+from ._lib import AttnDesc, GemmDesc, PagedAppendDesc, PagedAttnDesc
 
 BF16 = torch.bfloat16
 
@@ -821,6 +821,226 @@ def mha_packed_qkv(qkv, out, n_views, seq, heads, head_dim, scale=None,
         kv_splits=kv_splits)
     run_attention(d)
     return out
+
+
+# ---------------------------------------------------------------------------
+# Paged key/value cache
+# ---------------------------------------------------------------------------
+class PagedKV:
+    """Pages of a key/value cache that many sequences share: ``k``
+    [n_pages, kv_heads, page_size, head_dim] and ``v`` [n_pages, kv_heads,
+    head_dim, page_size] (transposed, keys contiguous), both contiguous;
+    bf16, or uint8 holding OCP e4m3fn bytes with fp32 ``k_scale`` /
+    ``v_scale`` [kv_heads] (value = scale * e4m3(byte)).  page_size is a
+    power of two, 16 .. 1024; head_dim 64, 128 or 256.  Which page belongs to
+    which sequence is the caller's page table (see paged_append)."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        e4m3 = k.dtype == torch.uint8
+        for t, nm in ((k, 'k'), (v, 'v')):
+            _check(t, nm, dtype=torch.uint8 if e4m3 else BF16)
+            if t.dim() != 4:
+                raise ValueError(f'{nm} must be 4-D')
+        n, h, page, d = k.shape
+        if tuple(v.shape) != (n, h, d, page):
+            raise ValueError(f'v must be {(n, h, d, page)} for k '
+                             f'{(n, h, page, d)}, got {tuple(v.shape)}')
+        if e4m3 != (k_scale is not None) or e4m3 != (v_scale is not None):
+            raise ValueError('k_scale and v_scale belong to an e4m3 (uint8) '
+                             'cache, which needs both')
+        for t, nm in ((k_scale, 'k_scale'), (v_scale, 'v_scale')):
+            if t is not None:
+                _check(t, nm, dtype=torch.float32)
+                if t.numel() != h:
+                    raise ValueError(f'{nm} must hold {h} values')
+        _same_device(k, v=v, k_scale=k_scale, v_scale=v_scale)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.e4m3 = e4m3
+        self.n_pages, self.kv_heads, self.page_size, self.head_dim = n, h, page, d
+
+    @staticmethod
+    def empty(n_pages, page_size, kv_heads, head_dim, device, k_scale=None,
+              v_scale=None):
+        """A pool of ``n_pages`` pages, e4m3 when scales are given.  Its
+        slots hold anything until paged_append writes them."""
+        dt = BF16 if k_scale is None else torch.uint8
+        return PagedKV(
+            torch.empty(n_pages, kv_heads, page_size, head_dim, dtype=dt, device=device),
+            torch.empty(n_pages, kv_heads, head_dim, page_size, dtype=dt, device=device),
+            k_scale, v_scale)
+
+
+def _same_device(ref, **others):
+    for nm, t in others.items():
+        if t is not None and t.device != ref.device:
+            raise ValueError(f'{nm} must be on {ref.device}, got {t.device}')
+
+
+def _int32(t, name, shape, ref):
+    """Pointer of a contiguous int32 tensor of ``shape`` on ref's device."""
+    if t is None:
+        return None
+    _check(t, name, dtype=torch.int32)
+    if tuple(t.shape) != shape:
+        raise ValueError(f'{name} must be {shape}, got {tuple(t.shape)}')
+    if t.device != ref.device:
+        raise ValueError(f'{name} must be on {ref.device}, got {t.device}')
+    return t.data_ptr()
+
+
+def _paged_batch(cache, page_table, kv_len, q_start, rows, ref):
+    """(page table pointer, row stride, kv_len, q_start, n_seqs, max_pages)."""
+    _check(page_table, 'page_table', dtype=torch.int32, contiguous=False)
+    if page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError('page_table must be 2-D with unit stride in its last dim')
+    n, pages = page_table.shape
+    _same_device(ref, page_table=page_table, cache=cache.k)
+    if q_start is None and rows != n:
+        raise ValueError(f'{rows} rows of {n} sequences need q_start')
+    stride = page_table.stride(0)
+    if n > 1 and stride < pages:
+        raise ValueError('page_table rows overlap')
+    return (page_table.data_ptr() or None, max(stride, pages),
+            _int32(kv_len, 'kv_len', (n,), ref),
+            _int32(q_start, 'q_start', (n + 1,), ref), n, pages)
+
+
+def _head_rows(t, name, heads, dim):
+    """(rows, row stride) of [rows, heads, dim] or [rows, heads * dim] with
+    the heads side by side."""
+    if t.dim() == 3 and tuple(t.shape[1:]) == (heads, dim):
+        side = (heads == 1 or t.stride(1) == dim) and t.stride(2) == 1
+    elif t.dim() == 2 and t.shape[1] == heads * dim:
+        side = t.stride(1) == 1
+    else:
+        raise ValueError(f'{name} must be [rows, {heads}, {dim}] or '
+                         f'[rows, {heads * dim}], got {tuple(t.shape)}')
+    if not side:
+        raise ValueError(f'{name}: the heads of a row must be contiguous')
+    n = t.shape[0]
+    if n < 2:
+        return n, heads * dim
+    if t.stride(0) < heads * dim:
+        raise ValueError(f'{name}: rows overlap')
+    return n, t.stride(0)
+
+
+def _call_on(name, desc, device):
+    """Entry point ``name`` on ``device`` and its current stream."""
+    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, ctypes.byref(desc), stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, ctypes.byref(desc), stream)
+
+
+def paged_append(qkv, cache, rope, page_table, kv_len, n_q_heads, q_out=None,
+                 q_start=None, positions=None):
+    """New tokens into a paged cache (fvx_paged_append): keys and values of
+    the Q|K|V product ``qkv`` (bf16 [rows, (n_q_heads + 2 kv_heads) *
+    head_dim], rotated pairs in columns 2i, 2i+1) go to their pages, keys
+    rotated; the rotated queries are returned (q_out, bf16 [rows, n_q_heads *
+    head_dim], new unless given; may be qkv's own columns; None without
+    query heads).
+
+    page_table int32 [n_seqs, max_pages]: token t of sequence b is slot
+    t % page_size of page page_table[b, t // page_size]; kv_len int32
+    [n_seqs]: lengths, the new tokens included; q_start int32 [n_seqs + 1]:
+    rows q_start[b] .. q_start[b + 1] - 1 are sequence b's last tokens (None:
+    one row per sequence).  rope fp32 [max_pos, head_dim / 2, 2] (rope_table),
+    read at ``positions`` (int32 [rows]) or at the tokens' own places.  The
+    device arrays are not read by the host; rows behind the last sequence,
+    and rows whose position is outside rope, are left as they were."""
+    _check(qkv, 'qkv', contiguous=False)
+    d, kv = cache.head_dim, cache.kv_heads
+    rows, ld = _head_rows(qkv, 'qkv', n_q_heads + 2 * kv, d)
+    _check(rope, 'rope', dtype=torch.float32)
+    if rope.dim() != 3 or tuple(rope.shape[1:]) != (d // 2, 2):
+        raise ValueError(f'rope must be [max_pos, {d // 2}, 2], got {tuple(rope.shape)}')
+    if q_out is None and n_q_heads:
+        q_out = torch.empty(rows, n_q_heads * d, dtype=BF16, device=qkv.device)
+    qp, ldq = None, 0
+    if q_out is not None:
+        _check(q_out, 'q_out', contiguous=False)
+        n, ldq = _head_rows(q_out, 'q_out', n_q_heads, d)
+        if n != rows:
+            raise ValueError(f'q_out must have {rows} rows, got {n}')
+        qp = q_out.data_ptr()
+    _same_device(qkv, rope=rope, q_out=q_out)
+    table, stride, lens, starts, n_seqs, pages = _paged_batch(
+        cache, page_table, kv_len, q_start, rows, qkv)
+    desc = PagedAppendDesc(
+        qkv.data_ptr(), ld, qp, ldq, cache.k.data_ptr(), cache.v.data_ptr(),
+        _ptr(cache.k_scale), _ptr(cache.v_scale), rope.data_ptr(), rope.shape[0],
+        _int32(positions, 'positions', (rows,), qkv), table, stride, lens, starts,
+        rows, n_seqs, pages, cache.n_pages, cache.page_size, n_q_heads, kv, d,
+        cache.e4m3)
+    _call_on('fvx_paged_append', desc, qkv.device)
+    return q_out
+
+
+def paged_attention(q, cache, page_table, kv_len, out=None, q_start=None,
+                    max_q=0, prefix_len=None, window=0, softcap=0.0,
+                    scale=None, workspace=None):
+    """Attention of the newest tokens of many sequences over their paged
+    cache (fvx_paged_attention): q bf16 [rows, q_heads, head_dim] (rotated,
+    paged_append's), q_heads a multiple of the cache's kv_heads; out like q
+    (new unless given) is returned.  page_table, kv_len, q_start: as for
+    paged_append, whose new tokens are in the cache by now.
+
+    A token at position t sees keys j <= t, all keys j < prefix_len[b]
+    (int32 [n_seqs]) and, with ``window``, only keys j > t - window.
+    ``softcap`` c > 0: scores c * tanh(s / c).  A token that sees nothing
+    gives zeros; rows behind the last sequence are left as they were.
+    ``max_q``: the most new tokens of one sequence when known (a hint).
+    workspace: uint8 of paged_attention_workspace_bytes, taken from the
+    allocator unless given; calls on different streams need their own."""
+    _check(q, 'q', contiguous=False)
+    if q.dim() != 3:
+        raise ValueError('q must be [rows, q_heads, head_dim]')
+    d, kv = cache.head_dim, cache.kv_heads
+    heads = q.shape[1]
+    rows, ldq = _head_rows(q, 'q', heads, d)
+    if out is None:
+        out = torch.empty(rows, heads, d, dtype=BF16, device=q.device)
+    _check(out, 'out', contiguous=False)
+    n, ldo = _head_rows(out, 'out', heads, d)
+    if n != rows:
+        raise ValueError(f'out must have {rows} rows, got {n}')
+    _same_device(q, out=out)
+    if q_start is None:
+        max_q = 1
+    table, stride, lens, starts, n_seqs, pages = _paged_batch(
+        cache, page_table, kv_len, q_start, rows, q)
+    desc = PagedAttnDesc(
+        q.data_ptr(), ldq, out.data_ptr(), ldo, cache.k.data_ptr(),
+        cache.v.data_ptr(), _ptr(cache.k_scale), _ptr(cache.v_scale), table, stride,
+        lens, starts, _int32(prefix_len, 'prefix_len', (n_seqs,), q), rows, n_seqs,
+        pages, max_q, cache.n_pages, cache.page_size, heads, kv, d, window,
+        d ** -0.5 if scale is None else scale, softcap, cache.e4m3)
+    if workspace is None:
+        workspace = torch.empty(_paged_ws_bytes(desc, q.device), dtype=torch.uint8,
+                                device=q.device)
+    else:
+        _check(workspace, 'workspace', dtype=torch.uint8)
+        _same_device(q, workspace=workspace)
+    desc.workspace, desc.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    _call_on('fvx_paged_attention', desc, q.device)
+    return out
+
+
+def _paged_ws_bytes(desc, device):
+    fn = _lib.load().fvx_paged_attention_workspace_bytes
+    if device.index == torch.cuda.current_device():
+        n = fn(ctypes.byref(desc))
+    else:
+        with torch.cuda.device(device):
+            n = fn(ctypes.byref(desc))
+    if n < 0:
+        raise ValueError(f'fvx_paged_attention: '
+                         f'{_lib.load().fvx_last_error().decode(errors="replace")} (status {n})')
+    return n
 
 
 # ---------------------------------------------------------------------------

@@ -692,6 +692,99 @@ int fvx_rtc_vjp_update(float* x, int64_t ldx, void* x_bf16, int64_t ldxb,
                        int64_t cols, int64_t period, float omt, float dt,
                        void* stream);
 
+/*
+ * A paged key/value cache and attention over it (no counterpart in the
+ * reference, whose caches are one contiguous tensor per sample): keys and
+ * values of many sequences of any lengths in one pool of pages, for decoding
+ * text beside or ahead of the action chunks.
+ *
+ * A page holds page_size (a power of two, 16 .. 1024) consecutive tokens of
+ * one sequence, for all key/value heads:
+ *   k [n_pages][kv_heads][page_size][head_dim]
+ *   v [n_pages][kv_heads][head_dim][page_size]   (transposed, like the value
+ *                                                 cache of fvx_attn_desc)
+ * in bf16, or (e4m3 = 1) in OCP e4m3fn bytes with one fp32 scale per key/value
+ * head: value = scale[head] * e4m3(byte).  Token t of sequence b is slot
+ * t % page_size of page page_table[b * table_stride + t / page_size].
+ * head_dim is 64, 128 or 256.
+ *
+ * A call works on the n_rows newest tokens ("rows") of n_seqs sequences:
+ * rows q_start[b] .. q_start[b + 1] - 1 are the last tokens of sequence b,
+ * whose length with them is kv_len[b]; q_start NULL: one row per sequence
+ * (n_rows == n_seqs).  Row i of n is at position kv_len[b] - n + i.
+ * page_table, kv_len, q_start, positions and prefix_len are device arrays
+ * (int32) that the host does not read: a captured graph follows their
+ * contents.  Values out of range never make a kernel leave its buffers: starts
+ * are clamped to n_rows, lengths to the table's capacity max_pages *
+ * page_size, and a page id outside [0, n_pages) is a page that does not exist
+ * -- nothing is written there and no row sees its keys.  Sequences may share
+ * pages that they only read.
+ *
+ * fvx_paged_append: rows of qkv are the Q|K|V product [q_heads | kv_heads |
+ * kv_heads] x head_dim (bf16; columns (2i, 2i+1) of a Q or K head are a
+ * rotated pair, the fvx_gemm QKV_ROPE order).  Queries and keys are rotated
+ * with rope[pos][i] = (cos, sin) (fp32, max_pos positions; pos = positions[row]
+ * or, NULL, the row's own position) in fp32 and rounded once: queries to bf16
+ * at q_out (NULL: not written; may be qkv itself), keys to the cache's type.
+ * e4m3: x / scale, to nearest even, at most 448 in magnitude.  A row that
+ * belongs to no sequence, or whose pos is outside [0, max_pos), is left as it
+ * was everywhere; one whose page does not exist writes its query only.  Rows
+ * of one call whose tokens share a slot (sequences that share a page they
+ * write) leave some of their values there.
+ */
+typedef struct fvx_paged_append_desc {
+  const void* qkv; int64_t ld_qkv; /* bf16, row stride in elements */
+  void* q_out; int64_t ld_q;
+  void* k; void* v;
+  const float* k_scale; const float* v_scale; /* [kv_heads], e4m3 only */
+  const float* rope; int64_t max_pos;
+  const int32_t* positions;        /* [n_rows] or NULL */
+  const int32_t* page_table; int64_t table_stride;
+  const int32_t* kv_len;           /* [n_seqs] */
+  const int32_t* q_start;          /* [n_seqs + 1] or NULL */
+  int64_t n_rows, n_seqs, max_pages;
+  int64_t n_pages, page_size, q_heads, kv_heads, head_dim;
+  int32_t e4m3;
+} fvx_paged_append_desc;
+
+int fvx_paged_append(const fvx_paged_append_desc* d, void* stream);
+
+/*
+ * fvx_paged_attention: o[row][head] = sum_j softmax_j(s_j) v_j with
+ * s_j = cap(scale q . k_j), cap(x) = softcap * tanh(x / softcap) (softcap 0:
+ * x), over the keys j that the row sees; query head h reads key/value head
+ * h / (q_heads / kv_heads).  The row at position t sees keys j < kv_len with
+ * j <= t or j < prefix_len[b] (NULL: 0) and, with window > 0, j > t - window.
+ * A row that sees no key (a position before the sequence's start, missing
+ * pages) is zero; rows that belong to no sequence are left as they were.
+ * What unwritten slots hold does not matter, infinities and NaN included.
+ * fp32 scores, statistics and sums; bf16 probabilities in the second product.
+ * max_q: a hint, the most rows of a sequence (0: unknown); any value gives
+ * the same sums, in an order that may differ.
+ * workspace: fvx_paged_attention_workspace_bytes(d) bytes, 16-byte aligned,
+ * of any contents; nothing in it is kept between calls, but calls that overlap
+ * (other streams) need workspaces of their own.
+ */
+typedef struct fvx_paged_attn_desc {
+  const void* q; int64_t ldq;      /* [n_rows][q_heads][head_dim] bf16 */
+  void* o; int64_t ldo;            /* like q; row strides in elements */
+  const void* k; const void* v;
+  const float* k_scale; const float* v_scale;
+  const int32_t* page_table; int64_t table_stride;
+  const int32_t* kv_len;
+  const int32_t* q_start;
+  const int32_t* prefix_len;       /* [n_seqs] or NULL */
+  int64_t n_rows, n_seqs, max_pages, max_q;
+  int64_t n_pages, page_size, q_heads, kv_heads, head_dim;
+  int64_t window;                  /* 0: none */
+  float scale, softcap;
+  int32_t e4m3;
+  void* workspace; int64_t workspace_bytes;
+} fvx_paged_attn_desc;
+
+int64_t fvx_paged_attention_workspace_bytes(const fvx_paged_attn_desc* d);
+int fvx_paged_attention(const fvx_paged_attn_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
