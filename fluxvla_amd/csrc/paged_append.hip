@@ -42,6 +42,17 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_sat(c), e4m3_sat(d), r, true);
 }
 
+// Four pairs (a, b) turned by (cos, sin): (a c - b s, b c + a s), every
+// operation rounded to fp32.
+__device__ __forceinline__ void rotate8(const float* f, const float* cs, float* w) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    w[e] = f[e] * cs[e] - f[e + 1] * cs[e + 1];
+    w[e + 1] = f[e + 1] * cs[e] + f[e] * cs[e + 1];
+  }
+}
+
 constexpr int kEndsLds = 1024;  // sequence ends held in LDS for the search
 
 // RB rows x one head (blockIdx.y: query heads, key heads, value heads).
@@ -135,11 +146,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
       const float cs[8] = {ra[0], ra[1], ra[2], ra[3], rb[0], rb[1], rb[2], rb[3]};
       float f[8], w[8];
       unpack8(x[u], f);
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        w[e] = __fsub_rn(__fmul_rn(f[e], cs[e]), __fmul_rn(f[e + 1], cs[e + 1]));
-        w[e + 1] = __fadd_rn(__fmul_rn(f[e + 1], cs[e]), __fmul_rn(f[e], cs[e + 1]));
-      }
+      rotate8(f, cs, w);
       if (is_q) {
         if (p.q_out) st8(p.q_out + (r0 + i) * p.ld_q + (int64_t)h * D + 8 * c, pack8(w));
         continue;

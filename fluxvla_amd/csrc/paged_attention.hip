@@ -36,8 +36,14 @@ struct PagedAttn {
   const int32_t* prefix_len;
   int32_t kv_heads, group, window;
   float scale, softcap;
+  // few rows: sequences of at most most_rows query rows per key/value head
+  int32_t most_rows;
   int32_t* rec;  // [n_wg][8] problems that cross workgroups
   float* part;   // [n_wg][2][16 rows x (D + 2)] partials
+  // many rows: the others; problems and key ranges of the launch
+  int32_t problems, splits;
+  int32_t* prec;  // [problems][4]
+  float* ppart;   // [problems][splits][rows x (D + 2)]
 };
 
 // Max / sum of the four lanes l, l ^ 16, l ^ 32, l ^ 48 (one query row's
@@ -139,7 +145,8 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttn p) {
   auto seq_units = [&](int b, int& per, int& tiles) {
     PagedSeq s;
     s.load(p, b);
-    tiles = (int)(((int64_t)s.n * G + kDecRows - 1) / kDecRows);
+    const int64_t rows = (int64_t)s.n * G;
+    tiles = rows <= p.most_rows ? (int)((rows + kDecRows - 1) / kDecRows) : 0;
     int lo, hi, x;
     s.keys(p, 0, lo, x);
     s.keys(p, s.n - 1, x, hi);
@@ -515,19 +522,554 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn p) {
 }
 
 // ---------------------------------------------------------------------------
+// Many rows per sequence: 32x32x16 MFMAs, keys and values through LDS
+// ---------------------------------------------------------------------------
+// Bound by the matrix cores and the exponentials.  A workgroup owns 128 NR
+// query rows of one key/value head, a wave 32 NR of them, and walks the keys
+// they see (or one of `splits` ranges of them) in tiles of 64.  Tiles arrive
+// in LDS by DMA, one barrier per tile, keys one tile ahead of values.  A wave
+// goes on in halves of 32 keys, three of which are in work at once: the
+// scores of half h + 1 and the output of half h - 1 are on the matrix cores
+// while the exponentials of half h are taken.
+//
+// Scores refer to a row's reference, its running maximum when that last rose
+// by more than kSlack above it: probabilities stay below 2^kSlack, and the
+// output is rescaled a few times per row, not once per tile.
+constexpr int kProTile = 64;
+constexpr int kProPages = 2048;  // page ids held in LDS at a time
+constexpr float kSlack = 8.f;
+
+// 16 bytes per lane from a 64-bit address straight into LDS (lane l's at lds +
+// 16 l); waited for with wait_vmcnt, like load_lds16.
+__device__ __forceinline__ void load_lds16_at(const void* a, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(a)
+               : "memory");
+}
+
+template <int D, bool F8>
+struct ProShape {
+  static constexpr int NR = D == 256 ? 1 : 2;   // 32-row groups per wave
+  static constexpr int BM = 128 * NR;           // rows per workgroup
+  static constexpr int ES = F8 ? 1 : 2;
+  static constexpr int KROW = D * ES;           // bytes of a key in LDS
+  static constexpr int VROW = kProTile * ES;    // bytes of a dim in LDS
+  static constexpr int TB = kProTile * D * ES;  // bytes of a tile of keys (of values)
+  static constexpr int NDB = D / 32;            // output blocks
+  static constexpr int NS = D / 16;             // MFMA steps of a score
+  static constexpr int PF = BM * (D + 2);       // floats of a partial
+};
+
+// 16-byte slot of logical chunk c of LDS row `row` (RB bytes long): rows that
+// lanes read together lie in different banks.
+template <int RB>
+__device__ __forceinline__ int swz(int row, int c) {
+  constexpr int RP = RB >= 256 ? 1 : 256 / RB, M = RB / 16 < 16 ? RB / 16 - 1 : 15;
+  return c ^ ((row / RP) & M);
+}
+
+// Problem `item` of the launch: the tiles of BM rows of the sequences with
+// more than most_rows rows, key/value head fastest, a sequence's last tile
+// (which sees most keys) first.  Returns false past the last one.
+template <int BM>
+__device__ bool find_tile(const PagedAttn& p, int item, int64_t* scan, int* found, int& b, int& t,
+                          int& h) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int each = (p.b.n_seqs + 255) / 256, first = tid * each;
+  auto tiles = [&](int s) {
+    int q0, n;
+    paged_rows(p.b, s, q0, n);
+    const int64_t rows = (int64_t)n * p.group;
+    return rows > p.most_rows ? (int)((rows + BM - 1) / BM) : 0;
+  };
+  int64_t mine = 0;
+  for (int i = 0; i < each; ++i)
+    if (first + i < p.b.n_seqs) mine += tiles(first + i);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t v = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 63) scan[wave] = incl;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i < wave) before += scan[i];
+    total += scan[i];
+  }
+  const int want = item / p.kv_heads;
+  h = item - want * p.kv_heads;
+  if (want >= total) return false;
+  int64_t at = before + incl - mine;
+  if (want >= at && want < at + mine) {
+    int s = first, n;
+    for (;; ++s) {
+      n = tiles(s);
+      if (want < at + n) break;
+      at += n;
+    }
+    found[0] = s;
+    found[1] = n - 1 - (int)(want - at);
+  }
+  __syncthreads();
+  b = __builtin_amdgcn_readfirstlane(found[0]);
+  t = __builtin_amdgcn_readfirstlane(found[1]);
+  return true;
+}
+
+template <int D, bool F8, bool CAP>
+__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(PagedAttn p) {
+  using S = ProShape<D, F8>;
+  constexpr int NR = S::NR;
+  __shared__ __align__(16) unsigned char smem[4 * S::TB];
+  __shared__ int sPid[kProPages + 4];
+  __shared__ int64_t sScan[4];
+  __shared__ int sFound[2];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int qi = lane & 31, hh = lane >> 5;
+  const int prob = blockIdx.x, split = blockIdx.y;
+  const int lg = p.b.lg_page, G = p.group;
+  int b, rt, h;
+  if (!find_tile<S::BM>(p, prob, sScan, sFound, b, rt, h)) {
+    if (split == 0 && tid == 0 && p.splits > 1) p.prec[prob * 4] = -1;
+    return;
+  }
+  PagedSeq s;
+  s.load(p, b);
+  const int all = s.n * G;
+  const int r_tile = rt * S::BM, rows = all - r_tile < S::BM ? all - r_tile : S::BM;
+  int lo_min, lo_tile, hi_tile, hi_max;
+  s.keys(p, r_tile / G, lo_min, hi_tile);
+  s.keys(p, (r_tile + rows - 1) / G, lo_tile, hi_max);
+  // tiles of this key range
+  int t0 = lo_min / kProTile, t1 = (hi_max + kProTile - 1) / kProTile;
+  if (t1 < t0) t1 = t0;
+  {
+    const int64_t n = t1 - t0;
+    t1 = t0 + (int)(n * (split + 1) / p.splits);
+    t0 = t0 + (int)(n * split / p.splits);
+  }
+
+  // this wave's rows: those past the tile's last repeat it and store nothing
+  const int r_wave = r_tile + 32 * NR * w;
+  const bool active = 32 * NR * w < rows;
+  int lo[NR], hi[NR], tok[NR], head[NR];
+  bf16x8 qf[NR][S::NS];
+  // a negative scale turns the queries' signs (exact), a zero one clears
+  // them: the scores' maximum can then be taken before scaling
+  const float ks = F8 ? p.k_scale[h] : 1.f;
+  const float raw = p.scale * ks;
+  const float sc = (raw == 0.f ? 1.f : fabsf(raw)) * (CAP ? 2.f / p.softcap : 1.f) * kLog2e;
+  const float cap = CAP ? p.softcap * kLog2e : 0.f;
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int i = 32 * NR * w + 32 * n + qi;
+    const int r = r_tile + (i < rows ? i : rows - 1);
+    tok[n] = r / G;
+    head[n] = h * G + r - tok[n] * G;
+    s.keys(p, tok[n], lo[n], hi[n]);
+    const bf16_t* qr = p.q + (int64_t)(s.q0 + tok[n]) * p.ldq + (int64_t)head[n] * D;
+#pragma unroll
+    for (int x = 0; x < S::NS; ++x) {
+      qf[n][x] = ld8(qr + (F8 ? 32 * (x >> 1) + 16 * hh + 8 * (x & 1) : 16 * x + 8 * hh));
+      if (raw <= 0.f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[n][x].w[e] = raw == 0.f ? 0u : qf[n][x].w[e] ^ 0x80008000u;
+    }
+  }
+  // the wave's rows all see keys [lo_max, hi_min)
+  int lo_max = lo_tile, hi_min = hi_tile;
+  if (active) {
+    int x;
+    const int last = r_wave + 32 * NR - 1 < r_tile + rows - 1 ? r_wave + 32 * NR - 1
+                                                              : r_tile + rows - 1;
+    s.keys(p, r_wave / G, x, hi_min);
+    s.keys(p, last / G, lo_max, x);
+  }
+
+  f32x16_t o[NR][S::NDB], sa[2][NR];
+  float ref[NR], l_run[NR];
+  bf16x8 pt[NR][2];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    ref[n] = -INFINITY;
+    l_run[n] = 0.f;
+#pragma unroll
+    for (int db = 0; db < S::NDB; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[n][db][e] = 0.f;
+  }
+
+  const uint32_t lds = lds_addr(smem);
+  // keys of tile t into K buffer t & 1, values into V buffer t & 1
+  constexpr int LPW = S::TB / 1024 / 4;  // DMA instructions per wave
+  int pg0 = 0;
+  auto load_k = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const int c = 64 * (LPW * w + i) + lane, row = c / (S::KROW / 16);
+      const int ch = swz<S::KROW>(row, c % (S::KROW / 16));
+      const int key = t * kProTile + row, id = sPid[(key >> lg) - pg0];
+      const unsigned char* a =
+          p.k + ((((int64_t)(id < 0 ? 0 : id) * p.kv_heads + h) << lg) + (key & ((1 << lg) - 1))) *
+                    S::KROW + 16 * ch;
+      load_lds16_at(a, lds + (t & 1) * S::TB + 1024 * (LPW * w + i));
+    }
+  };
+  auto load_v = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const int c = 64 * (LPW * w + i) + lane, d = c / (S::VROW / 16);
+      const int ch = swz<S::VROW>(d, c % (S::VROW / 16));
+      const int key = t * kProTile + ch * (16 / S::ES), id = sPid[(key >> lg) - pg0];
+      const unsigned char* a =
+          p.v + (((((int64_t)(id < 0 ? 0 : id) * p.kv_heads + h) * D + d) << lg) +
+                 (key & ((1 << lg) - 1))) * S::ES;
+      load_lds16_at(a, lds + (2 + (t & 1)) * S::TB + 1024 * (LPW * w + i));
+    }
+  };
+  // values that no row of the tile sees (unwritten slots, missing pages) may
+  // be anything: they are cleared in LDS, by the wave that loaded them
+  auto clear_v = [&](int t, bool missing) {
+    if (t * kProTile >= lo_min && (t + 1) * kProTile <= hi_max && !missing) return;
+#pragma unroll 1
+    for (int i = 0; i < LPW; ++i) {
+      const int c = 64 * (LPW * w + i) + lane, d = c / (S::VROW / 16);
+      const int key = t * kProTile + swz<S::VROW>(d, c % (S::VROW / 16)) * (16 / S::ES);
+      const bool gone = sPid[(key >> lg) - pg0] < 0;
+      bf16x8* x = (bf16x8*)(smem + (2 + (t & 1)) * S::TB + 16 * c);
+      bf16x8 v = *x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t keep = 0;
+#pragma unroll
+        for (int y = 0; y < 4 / S::ES; ++y) {
+          const int k = key + e * (4 / S::ES) + y;
+          if (k >= lo_min && k < hi_max && !gone) keep |= (F8 ? 0xffu : 0xffffu) << (8 * S::ES * y);
+        }
+        v.w[e] &= keep;
+      }
+      *x = v;
+    }
+  };
+  // does tile t hold a missing page?
+  auto missing_page = [&](int t) {
+    const int k = t * kProTile + lane;
+    return __any(sPid[(k >> lg) - pg0] < 0) != 0;
+  };
+
+  const int kperm = F8 ? 16 * ((qi >> 2) & 1) + 8 * (qi >> 4) + 4 * ((qi >> 3) & 1) + (qi & 3)
+                       : 16 * (qi >> 4) + 8 * ((qi >> 2) & 1) + 4 * ((qi >> 3) & 1) + (qi & 3);
+  // S^T of half hf of tile t
+  auto scores = [&](f32x16_t* d, int t, int hf) {
+    const unsigned char* base = smem + (t & 1) * S::TB;
+    const int row = 32 * hf + kperm;
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) d[n][e] = 0.f;
+    if constexpr (F8) {
+#pragma unroll
+      for (int x = 0; x < S::NS / 2; ++x) {
+        const bf16x8 kk = *(const bf16x8*)(base + row * S::KROW + 16 * swz<S::KROW>(row, 2 * x + hh));
+        const bf16x8 a = e4m3x8_to_bf16(kk.w[0], kk.w[1]), c = e4m3x8_to_bf16(kk.w[2], kk.w[3]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) d[n] = mfma32x32x16(a, qf[n][2 * x], d[n]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) d[n] = mfma32x32x16(c, qf[n][2 * x + 1], d[n]);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < S::NS; ++x) {
+        const bf16x8 a = *(const bf16x8*)(base + row * S::KROW + 16 * swz<S::KROW>(row, 2 * x + hh));
+#pragma unroll
+        for (int n = 0; n < NR; ++n) d[n] = mfma32x32x16(a, qf[n][x], d[n]);
+      }
+    }
+  };
+  // O^T += V^T P^T of half hf of tile t
+  auto output = [&](int t, int hf) {
+    const unsigned char* base = smem + (2 + (t & 1)) * S::TB;
+    if constexpr (F8) {
+#pragma unroll
+      for (int db = 0; db < S::NDB; ++db) {
+        const int d = 32 * db + qi;
+        const bf16x8 vv = *(const bf16x8*)(base + d * S::VROW + 16 * swz<S::VROW>(d, 2 * hf + hh));
+        const bf16x8 a = e4m3x8_to_bf16(vv.w[0], vv.w[1]), c = e4m3x8_to_bf16(vv.w[2], vv.w[3]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) o[n][db] = mfma32x32x16(a, pt[n][0], o[n][db]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) o[n][db] = mfma32x32x16(c, pt[n][1], o[n][db]);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int db = 0; db < S::NDB; ++db) {
+          const int d = 32 * db + qi;
+          const bf16x8 a =
+              *(const bf16x8*)(base + d * S::VROW + 16 * swz<S::VROW>(d, 4 * hf + 2 * u + hh));
+#pragma unroll
+          for (int n = 0; n < NR; ++n) o[n][db] = mfma32x32x16(a, pt[n][u], o[n][db]);
+        }
+    }
+  };
+  // Half hf of tile t: scores in sa[hf]; the next half's scores go to
+  // sa[hf ^ 1], the previous half's probabilities are in pt.
+  auto half = [&](int t, auto hfc, bool missing) {
+    constexpr int hf = decltype(hfc)::value;
+    f32x16_t* sv = sa[hf];
+    const int k0 = t * kProTile + 32 * hf;
+    const bool edge = k0 < lo_max || k0 + 32 > hi_min || missing;
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int key = k0 + (F8 ? 16 * hh + e : 16 * (e >> 3) + 8 * hh + (e & 7));
+        const bool gone = missing && sPid[(key >> lg) - pg0] < 0;
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+          if (key < lo[n] || key >= hi[n] || gone) sv[n][e] = -INFINITY;
+      }
+    }
+    float mb[NR];
+    bool up = false;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float m = sv[n][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) m = fmaxf(m, sv[n][e]);
+      m = half_pair_max(m) * sc;
+      if (CAP)
+        m = m == -INFINITY ? m : cap - 2.f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(m) + 1.f);
+      mb[n] = m;
+      up = up || m > ref[n] + kSlack;
+    }
+    if (__any(up)) {
+      // the probabilities not yet in the output follow it to the new
+      // reference (a second rounding to bf16, on the halves where it rises)
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const float nr = fmaxf(ref[n], mb[n]);
+        const float f = ref[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref[n] - nr);
+        ref[n] = nr;
+        l_run[n] *= f;
+#pragma unroll
+        for (int db = 0; db < S::NDB; ++db)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[n][db][e] *= f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float x[8];
+          unpack8(pt[n][u], x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= f;
+          pt[n][u] = pack8(x);
+        }
+      }
+    }
+    output(hf ? t : t - 1, hf ^ 1);
+    scores(sa[hf ^ 1], hf ? t + 1 : t, hf ^ 1);
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const float nm = ref[n] == -INFINITY ? 0.f : -ref[n];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float pv[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = sv[n][8 * u + e];
+          if (CAP) {
+            const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * sc) + 1.f);
+            pv[e] = __builtin_amdgcn_exp2f(fmaf(-2.f * cap, r, cap + nm));
+            if (x == -INFINITY) pv[e] = 0.f;
+          } else {
+            pv[e] = __builtin_amdgcn_exp2f(fmaf(x, sc, nm));
+          }
+          l_run[n] += pv[e];
+        }
+        pt[n][u] = pack8(pv);
+      }
+    }
+  };
+
+  const int CT = kProPages * 16 / kProTile;  // tiles per walk (pages hold 16 tokens or more)
+  for (int c0 = t0; c0 < t1; c0 += CT) {
+    const int c1 = c0 + CT < t1 ? c0 + CT : t1;
+    pg0 = (int)(((int64_t)c0 * kProTile) >> lg);
+    const int pg1 = (int)(((int64_t)c1 * kProTile - 1) >> lg);
+    __syncthreads();
+    for (int i = tid; i <= pg1 - pg0; i += 256) sPid[i] = paged_page(p.b, b, pg0 + i);
+    // the first half's "previous" values: zeros (with zero probabilities)
+    for (int i = tid; i < S::TB / 16; i += 256)
+      *(bf16x8*)(smem + (2 + ((c0 + 1) & 1)) * S::TB + 16 * i) = zero8();
+#pragma unroll
+    for (int n = 0; n < NR; ++n) pt[n][0] = pt[n][1] = zero8();
+    __syncthreads();
+    load_k(c0);
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (c0 + 1 < c1) load_k(c0 + 1);
+    load_v(c0);
+    if (active) scores(sa[0], c0, 0);
+    for (int t = c0; t < c1; ++t) {
+      const bool missing = missing_page(t);
+      if (active) half(t, IntC<0>{}, missing);
+      wait_vmcnt<0>();
+      clear_v(t, missing);
+      // everyone's keys of tile t + 1 and values of tile t are there, and
+      // the keys of tile t and the values of tile t - 1 have been used
+      __syncthreads();
+      if (t + 2 < c1) load_k(t + 2);
+      if (t + 1 < c1) load_v(t + 1);
+      if (active) half(t, IntC<1>{}, missing);
+    }
+    if (active) output(c1 - 1, 1);
+  }
+
+  if (!active && p.splits == 1) return;
+  const float vs = F8 ? p.v_scale[h] : 1.f;
+  float* part = p.ppart + ((int64_t)prob * p.splits + split) * S::PF;
+  if (p.splits > 1 && split == 0 && tid == 0) {
+    p.prec[prob * 4] = rows;
+    p.prec[prob * 4 + 1] = s.q0;
+    p.prec[prob * 4 + 2] = r_tile;
+    p.prec[prob * 4 + 3] = h;
+  }
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int i = 32 * NR * w + 32 * n + qi;
+    const float l = half_pair_sum(l_run[n]);
+    if (i >= rows) continue;
+    if (p.splits == 1) {
+      const float inv = l > 0.f ? vs / l : 0.f;
+      bf16_t* row = p.o + (int64_t)(s.q0 + tok[n]) * p.ldo + (int64_t)head[n] * D + 4 * hh;
+#pragma unroll
+      for (int db = 0; db < S::NDB; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint2 v;
+          v.x = f2bf2(o[n][db][4 * j] * inv, o[n][db][4 * j + 1] * inv);
+          v.y = f2bf2(o[n][db][4 * j + 2] * inv, o[n][db][4 * j + 3] * inv);
+          *(uint2*)(row + 32 * db + 8 * j) = v;
+        }
+    } else {
+      float* row = part + i * D + 4 * hh;
+#pragma unroll
+      for (int db = 0; db < S::NDB; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *(f32x4_t*)(row + 32 * db + 8 * j) =
+              f32x4_t{o[n][db][4 * j] * vs, o[n][db][4 * j + 1] * vs, o[n][db][4 * j + 2] * vs,
+                      o[n][db][4 * j + 3] * vs};
+      if (hh == 0) {
+        part[S::BM * D + i] = ref[n];
+        part[S::BM * D + S::BM + i] = l;
+      }
+    }
+  }
+}
+
+// The key ranges of a problem together, in their order: rows 16 blockIdx.y
+// ... of problem blockIdx.x.
+template <int D>
+__global__ __launch_bounds__(256) void paged_prompt_merge_kernel(PagedAttn p) {
+  using S = ProShape<D, false>;
+  const int prob = blockIdx.x, rows = p.prec[prob * 4];
+  if ((int)blockIdx.y * 16 >= rows) return;
+  const int q0 = p.prec[prob * 4 + 1], r_tile = p.prec[prob * 4 + 2], h = p.prec[prob * 4 + 3];
+  const float* part = p.ppart + (int64_t)prob * p.splits * S::PF;
+  for (int c = threadIdx.x; c < 16 * (D / 4); c += 256) {
+    const int i = blockIdx.y * 16 + c / (D / 4), d0 = (c % (D / 4)) * 4;
+    if (i >= rows) break;
+    float top = -INFINITY;
+    for (int k = 0; k < p.splits; ++k) top = fmaxf(top, part[(int64_t)k * S::PF + S::BM * D + i]);
+    f32x4_t a = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < p.splits; ++k) {
+      const float* x = part + (int64_t)k * S::PF;
+      const float m = x[S::BM * D + i];
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+      const f32x4_t t = *(const f32x4_t*)(x + i * D + d0);
+      l += f * x[S::BM * D + S::BM + i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] += f * t[e];
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int r = r_tile + i, tk = r / p.group;
+    uint2 v;
+    v.x = f2bf2(a[0] * inv, a[1] * inv);
+    v.y = f2bf2(a[2] * inv, a[3] * inv);
+    *(uint2*)(p.o + (int64_t)(q0 + tk) * p.ldo + (int64_t)(h * p.group + r - tk * p.group) * D + d0) = v;
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 // Workgroups of the decode kernel: as many as run at once (two per CU by
 // registers).
 static int decode_wgs() { return 2 * device_cus(); }
 
-static int64_t decode_ws_bytes(int64_t d, int n_wg) {
-  return (int64_t)n_wg * 8 * 4 + (int64_t)n_wg * 2 * kDecRows * (d + 2) * 4;
+// Which kernels a call launches, their grids and their parts of the
+// workspace.  The host knows the number of rows and sequences and, as a hint,
+// the most rows of one sequence, not who has how many.
+struct PagedPlan {
+  bool few, many;          // kernels launched
+  int most_rows;           // query rows up to which a sequence is the few kernel's
+  int n_wg;                // few: workgroups
+  int64_t problems;        // many: upper bound of the problems
+  int splits;
+  int64_t rec, part, prec, ppart, bytes;  // workspace offsets
+};
+
+static PagedPlan paged_plan(const fvx_paged_attn_desc* d) {
+  PagedPlan a = {};
+  const int64_t G = d->q_heads / d->kv_heads;
+  const int64_t most = d->q_start ? d->max_q : 1;
+  a.many = most == 0 || most * G > kDecRows;
+  // every sequence has most rows: none is left to the few kernel
+  a.few = !a.many || most == 0 || d->n_rows != d->n_seqs * most;
+  a.most_rows = !a.many ? 0x7fffffff : (a.few ? kDecRows : 0);
+  a.n_wg = a.few ? decode_wgs() : 0;
+  a.rec = 0;
+  a.part = (int64_t)a.n_wg * 32;
+  a.prec = a.part + (int64_t)a.n_wg * 2 * kDecRows * (d->head_dim + 2) * 4;
+  a.ppart = a.bytes = a.prec;
+  if (a.many) {
+    const int64_t bm = d->head_dim == 256 ? 128 : 256;
+    a.problems = (d->n_rows * G / bm + (d->n_seqs < d->n_rows ? d->n_seqs : d->n_rows)) * d->kv_heads;
+    // one workgroup per CU: with fewer problems their keys are split
+    const int64_t s = device_cus() / a.problems;
+    a.splits = s < 1 ? 1 : (int)s;
+    if (a.splits > 1) {
+      a.ppart = a.prec + (a.problems * 16 + 15) / 16 * 16;
+      a.bytes = a.ppart + a.problems * a.splits * bm * (d->head_dim + 2) * 4;
+    }
+  }
+  return a;
 }
 
 template <int D>
-static void launch_decode(const PagedAttn& p, bool f8, bool cap, int n_wg, unsigned ry,
-                          hipStream_t s) {
+static void launch_many(const PagedAttn& p, bool f8, bool cap, hipStream_t s) {
+  const dim3 grid((unsigned)p.problems, (unsigned)p.splits), block(256);
+  if (f8 && cap) hipLaunchKernelGGL((paged_prompt_kernel<D, true, true>), grid, block, 0, s, p);
+  else if (f8) hipLaunchKernelGGL((paged_prompt_kernel<D, true, false>), grid, block, 0, s, p);
+  else if (cap) hipLaunchKernelGGL((paged_prompt_kernel<D, false, true>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((paged_prompt_kernel<D, false, false>), grid, block, 0, s, p);
+  if (p.splits > 1)
+    hipLaunchKernelGGL((paged_prompt_merge_kernel<D>),
+                       dim3((unsigned)p.problems, ProShape<D, false>::BM / 16), block, 0, s, p);
+}
+
+template <int D>
+static void launch_few(const PagedAttn& p, bool f8, bool cap, int n_wg, unsigned ry,
+                       hipStream_t s) {
   const dim3 grid((unsigned)n_wg), block(256);
   if (f8 && cap) hipLaunchKernelGGL((paged_decode_kernel<D, true, true>), grid, block, 0, s, p);
   else if (f8) hipLaunchKernelGGL((paged_decode_kernel<D, true, false>), grid, block, 0, s, p);
@@ -577,7 +1119,7 @@ extern "C" int64_t fvx_paged_attention_workspace_bytes(const fvx_paged_attn_desc
   const int st = check_paged_attention(d);
   if (st) return st;
   if (d->n_rows == 0 || d->n_seqs == 0) return 0;
-  return decode_ws_bytes(d->head_dim, decode_wgs());
+  return paged_plan(d).bytes;
 }
 
 extern "C" int fvx_paged_attention(const fvx_paged_attn_desc* d, void* stream) {
@@ -599,10 +1141,12 @@ extern "C" int fvx_paged_attention(const fvx_paged_attn_desc* d, void* stream) {
               FVX_ERR_SHAPE,
               "paged_attention: ldq and ldo must hold q_heads * head_dim values, table_stride "
               "max_pages entries");
-  const int n_wg = decode_wgs();
-  FVX_REQUIRE(d->workspace && d->workspace_bytes >= decode_ws_bytes(d->head_dim, n_wg),
-              FVX_ERR_WORKSPACE, "paged_attention: workspace of %lld bytes required",
-              (long long)decode_ws_bytes(d->head_dim, n_wg));
+  const PagedPlan plan = paged_plan(d);
+  FVX_REQUIRE(plan.problems < 1ll << 31, FVX_ERR_SHAPE,
+              "paged_attention: too many rows and sequences for one launch");
+  FVX_REQUIRE(plan.bytes == 0 || (d->workspace && d->workspace_bytes >= plan.bytes),
+              FVX_ERR_WORKSPACE,
+              "paged_attention: workspace of %lld bytes required", (long long)plan.bytes);
   PagedAttn p;
   p.b.page_table = d->page_table;
   p.b.table_stride = d->table_stride;
@@ -627,14 +1171,26 @@ extern "C" int fvx_paged_attention(const fvx_paged_attn_desc* d, void* stream) {
   p.window = (int)d->window;
   p.scale = d->scale;
   p.softcap = d->softcap;
-  p.part = (float*)d->workspace;
-  p.rec = (int32_t*)(p.part + (int64_t)n_wg * 2 * kDecRows * (d->head_dim + 2));
+  char* ws = (char*)d->workspace;
+  p.most_rows = plan.most_rows;
+  p.rec = (int32_t*)(ws + plan.rec);
+  p.part = (float*)(ws + plan.part);
+  p.problems = (int)plan.problems;
+  p.splits = plan.splits;
+  p.prec = (int32_t*)(ws + plan.prec);
+  p.ppart = (float*)(ws + plan.ppart);
   hipStream_t s = (hipStream_t)stream;
   const bool cap = d->softcap > 0.f;
-  const int64_t most = p.group * (d->max_q > 0 ? d->max_q : 16);
-  const unsigned ry = (unsigned)(most < kDecRows ? most : kDecRows);
-  if (d->head_dim == 64) launch_decode<64>(p, d->e4m3 != 0, cap, n_wg, ry, s);
-  else if (d->head_dim == 128) launch_decode<128>(p, d->e4m3 != 0, cap, n_wg, ry, s);
-  else launch_decode<256>(p, d->e4m3 != 0, cap, n_wg, ry, s);
+  const int64_t most = (d->q_start ? d->max_q : 1) * p.group;
+  const unsigned ry = (unsigned)(most > 0 && most < kDecRows ? most : kDecRows);
+#define FVX_PAGED(D)                                                        \
+  do {                                                                      \
+    if (plan.many) launch_many<D>(p, d->e4m3 != 0, cap, s);                 \
+    if (plan.few) launch_few<D>(p, d->e4m3 != 0, cap, plan.n_wg, ry, s);    \
+  } while (0)
+  if (d->head_dim == 64) FVX_PAGED(64);
+  else if (d->head_dim == 128) FVX_PAGED(128);
+  else FVX_PAGED(256);
+#undef FVX_PAGED
   return launch_status("paged_attention");
 }

@@ -243,6 +243,12 @@ def test_max_q_is_only_a_hint(cuda, new, max_q):
     _attend(cuda, [90, 75], new, 8, 1, 64, 16, single=False, max_q=max_q)
 
 
+def test_equal_prompts_need_no_workspace(cuda):
+    # more problems than CUs, none of few rows: nothing to join
+    announce('paged prompt without workspace')
+    _attend(cuda, [20 + i for i in range(16)], [20] * 16, 16, 16, 64, 16)
+
+
 def test_more_new_tokens_than_length(cuda):
     # the first rows lie before the sequence's start: they see nothing
     announce('paged prompt rows before the start')
@@ -445,6 +451,23 @@ def test_append_many_sequences(cuda):
     announce('paged append 1500 sequences')
     lens = [(i * 37) % 50 + 2 for i in range(1500)]
     _append_check(cuda, lens, [i % 3 for i in range(1500)], 2, 1, 64, 16)
+
+
+def test_append_rounds_like_separate_operations(cuda):
+    # two products and a sum, each in fp32, then one rounding: bit for bit
+    announce('paged append rounding')
+    qkv = torch.randn(500, 4 * 128, generator=torch.Generator().manual_seed(6)).bfloat16().to(cuda)
+    cache = K.PagedKV.empty(32, 16, 1, 128, cuda)
+    rope = K.rope_table(500, 128, device=cuda)
+    lens = torch.tensor([500], dtype=torch.int32, device=cuda)
+    starts = torch.tensor([0, 500], dtype=torch.int32, device=cuda)
+    q = K.paged_append(qkv, cache, rope, torch.arange(32, dtype=torch.int32, device=cuda)[None],
+                       lens, 2, q_start=starts)
+    x = qkv.float().view(500, 4, 128)
+    a, b, c, s = x[..., 0::2], x[..., 1::2], rope[:, None, :, 0], rope[:, None, :, 1]
+    want = torch.stack((a * c - b * s, b * c + a * s), -1).flatten(-2).bfloat16()
+    assert torch.equal(q, want[:, :2].flatten(1))
+    assert torch.equal(cache.k[:, 0].flatten(0, 1)[:500], want[:, 2])
 
 
 def test_append_e4m3_saturates(cuda):
