@@ -536,16 +536,32 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn p) {
 // by more than kSlack above it: probabilities stay below 2^kSlack, and the
 // output is rescaled a few times per row, not once per tile.
 constexpr int kProTile = 64;
-constexpr int kProPages = 2048;  // page ids held in LDS at a time
+// Page ids in LDS: two runs of kProRun tiles (of at most 4 pages each), the
+// second of which is refilled while the first is walked.
+constexpr int kProRun = 128;
+constexpr int kProPages = 2 * kProRun * kProTile / 16;
 constexpr float kSlack = 8.f;
 
-// 16 bytes per lane from a 64-bit address straight into LDS (lane l's at lds +
-// 16 l); waited for with wait_vmcnt, like load_lds16.
+// 16 bytes per lane from 64-bit addresses, or from a uniform base and 32-bit
+// offsets, straight into LDS (lane l's at lds + 16 l); waited for with
+// wait_vmcnt, like load_lds16.
 __device__ __forceinline__ void load_lds16_at(const void* a, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
                :
                : "s"(lds), "v"(a)
                : "memory");
+}
+__device__ __forceinline__ void load_lds16_at(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory");
+}
+
+// l + the two bf16 values of w, as the second product reads them.
+__device__ __forceinline__ float add_pair(uint32_t w, float l) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w),
+                                         __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
 }
 
 template <int D, bool F8>
@@ -625,9 +641,9 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
   using S = ProShape<D, F8>;
   constexpr int NR = S::NR;
   __shared__ __align__(16) unsigned char smem[4 * S::TB];
-  __shared__ int sPid[kProPages + 4];
+  __shared__ int sPid[kProPages];
   __shared__ int64_t sScan[4];
-  __shared__ int sFound[2];
+  __shared__ int sFound[2], sMissing;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -692,9 +708,10 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
     s.keys(p, last / G, lo_max, x);
   }
 
+  // O^T, the scores of a tile's halves (sa[half]) and their probabilities
   f32x16_t o[NR][S::NDB], sa[2][NR];
+  bf16x8 pt[2][NR][2];
   float ref[NR], l_run[NR];
-  bf16x8 pt[NR][2];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     ref[n] = -INFINITY;
@@ -705,43 +722,92 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
       for (int e = 0; e < 16; ++e) o[n][db][e] = 0.f;
   }
 
+  // DMA: instruction L = LPW w + i (1 KiB) brings K rows RPK L .. or dims RPV L
+  // ... of a tile.  Its K rows share a page.  A tile's values share one when
+  // pages hold a tile or more; otherwise a lane's keys do, at a place in the
+  // page that is the same in every tile.
   const uint32_t lds = lds_addr(smem);
-  // keys of tile t into K buffer t & 1, values into V buffer t & 1
-  constexpr int LPW = S::TB / 1024 / 4;  // DMA instructions per wave
-  int pg0 = 0;
-  auto load_k = [&](int t) {
+  constexpr int LPW = S::TB / 1024 / 4;
+  constexpr int CK = S::KROW / 16, CV = S::VROW / 16, RPK = 64 / CK, RPV = 64 / CV;
+  constexpr int NV = LPW > 1 && !F8 ? 2 : 1;  // key chunks that differ over i
+  const int mask = (1 << lg) - 1;
+  const bool big_page = (1 << lg) >= kProTile;
+  const int64_t head_k = (int64_t)S::KROW << lg, head_v = ((int64_t)D * S::ES) << lg;  // bytes
+  uint32_t koff[LPW];
 #pragma unroll
-    for (int i = 0; i < LPW; ++i) {
-      const int c = 64 * (LPW * w + i) + lane, row = c / (S::KROW / 16);
-      const int ch = swz<S::KROW>(row, c % (S::KROW / 16));
-      const int key = t * kProTile + row, id = sPid[(key >> lg) - pg0];
-      const unsigned char* a =
-          p.k + ((((int64_t)(id < 0 ? 0 : id) * p.kv_heads + h) << lg) + (key & ((1 << lg) - 1))) *
-                    S::KROW + 16 * ch;
-      load_lds16_at(a, lds + (t & 1) * S::TB + 1024 * (LPW * w + i));
+  for (int i = 0; i < LPW; ++i)
+    koff[i] = (lane / CK) * S::KROW + 16 * swz<S::KROW>(RPK * (LPW * w + i) + lane / CK, lane % CK);
+  int vchunk[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) vchunk[i] = swz<S::VROW>(RPV * (LPW * w + i) + lane / CV, lane % CV);
+  const uint32_t vrow = ((uint32_t)(RPV * LPW * w + lane / CV) * S::ES) << lg;
+
+  bool missing = false;  // has a page so far not existed?
+  // the page of a token, -1 for none
+  auto page_of = [&](int key) { return sPid[(key >> lg) & (kProPages - 1)]; };
+  // ids of the pages of tiles [ta, ta + kProRun), by all threads
+  auto fill_ids = [&](int ta) {
+    const int first = (ta * kProTile) >> lg, n = (kProRun * kProTile) >> lg;
+    for (int i = tid; i < n; i += 256) {
+      const int id = paged_page(p.b, b, first + i);
+      sPid[(first + i) & (kProPages - 1)] = id;
+      if (id < 0 && (int64_t)(first + i) << lg < hi_max) sMissing = 1;
     }
   };
-  auto load_v = [&](int t) {
+  struct Ids {
+    int k[LPW], v[NV];
+  };
+  // page ids for load_k(tk) and load_v(tv), ahead of them
+  auto fetch_ids = [&](int tk, int tv) {
+    Ids d;
+#pragma unroll
+    for (int i = 0; i < LPW; ++i)
+      d.k[i] = page_of(tk * kProTile + RPK * (LPW * w + i));
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      d.v[i] = page_of(tv * kProTile + (big_page ? 0 : vchunk[i] * (16 / S::ES)));
+    return d;
+  };
+  auto load_k = [&](int t, const Ids& d) {
 #pragma unroll
     for (int i = 0; i < LPW; ++i) {
-      const int c = 64 * (LPW * w + i) + lane, d = c / (S::VROW / 16);
-      const int ch = swz<S::VROW>(d, c % (S::VROW / 16));
-      const int key = t * kProTile + ch * (16 / S::ES), id = sPid[(key >> lg) - pg0];
-      const unsigned char* a =
-          p.v + (((((int64_t)(id < 0 ? 0 : id) * p.kv_heads + h) * D + d) << lg) +
-                 (key & ((1 << lg) - 1))) * S::ES;
-      load_lds16_at(a, lds + (2 + (t & 1)) * S::TB + 1024 * (LPW * w + i));
+      const int L = LPW * w + i;
+      const int id = __builtin_amdgcn_readfirstlane(d.k[i] < 0 ? 0 : d.k[i]);
+      const int64_t at = ((int64_t)id * p.kv_heads + h) * head_k +
+                         ((t * kProTile + RPK * L) & mask) * S::KROW;
+      load_lds16_at(p.k + at, koff[i], lds + (t & 1) * S::TB + 1024 * L);
+    }
+  };
+  auto load_v = [&](int t, const Ids& d) {
+    if (big_page) {
+      const int id = __builtin_amdgcn_readfirstlane(d.v[0] < 0 ? 0 : d.v[0]);
+      const unsigned char* at = p.v + ((int64_t)id * p.kv_heads + h) * head_v +
+                                ((t * kProTile) & mask) * S::ES;
+#pragma unroll
+      for (int i = 0; i < LPW; ++i)
+        load_lds16_at(at, vrow + (((uint32_t)i * RPV * S::ES) << lg) + 16 * vchunk[i % NV],
+                      lds + (2 + (t & 1)) * S::TB + 1024 * (LPW * w + i));
+    } else {
+      const unsigned char* at[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        at[i] = p.v + ((int64_t)(d.v[i] < 0 ? 0 : d.v[i]) * p.kv_heads + h) * head_v + vrow +
+                ((vchunk[i] * (16 / S::ES)) & mask) * S::ES;
+#pragma unroll
+      for (int i = 0; i < LPW; ++i)
+        load_lds16_at(at[i % NV] + (((uint32_t)i * RPV * S::ES) << lg),
+                      lds + (2 + (t & 1)) * S::TB + 1024 * (LPW * w + i));
     }
   };
   // values that no row of the tile sees (unwritten slots, missing pages) may
   // be anything: they are cleared in LDS, by the wave that loaded them
-  auto clear_v = [&](int t, bool missing) {
+  auto clear_v = [&](int t) {
     if (t * kProTile >= lo_min && (t + 1) * kProTile <= hi_max && !missing) return;
 #pragma unroll 1
     for (int i = 0; i < LPW; ++i) {
-      const int c = 64 * (LPW * w + i) + lane, d = c / (S::VROW / 16);
-      const int key = t * kProTile + swz<S::VROW>(d, c % (S::VROW / 16)) * (16 / S::ES);
-      const bool gone = sPid[(key >> lg) - pg0] < 0;
+      const int c = 64 * (LPW * w + i) + lane, d = c / CV;
+      const int key = t * kProTile + swz<S::VROW>(d, c % CV) * (16 / S::ES);
+      const bool gone = page_of(key) < 0;
       bf16x8* x = (bf16x8*)(smem + (2 + (t & 1)) * S::TB + 16 * c);
       bf16x8 v = *x;
 #pragma unroll
@@ -757,178 +823,236 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
       *x = v;
     }
   };
-  // does tile t hold a missing page?
-  auto missing_page = [&](int t) {
-    const int k = t * kProTile + lane;
-    return __any(sPid[(k >> lg) - pg0] < 0) != 0;
-  };
 
+  // Operand fragments of a half, in the order of their products: output block
+  // pairs (bf16: steps u of both blocks; e4m3: both steps of a block in one
+  // read), then the scores' steps.  They go through a ring of registers, read
+  // kAhead before their products.
+  constexpr int NVR = F8 ? S::NDB : 2 * S::NDB;  // reads of values
+  constexpr int NKR = F8 ? S::NS / 2 : S::NS;    // reads of keys
+  constexpr int kRing = D == 64 ? 4 : 8, kAhead = D == 64 ? 3 : 6;
   const int kperm = F8 ? 16 * ((qi >> 2) & 1) + 8 * (qi >> 4) + 4 * ((qi >> 3) & 1) + (qi & 3)
                        : 16 * (qi >> 4) + 8 * ((qi >> 2) & 1) + 4 * ((qi >> 3) & 1) + (qi & 3);
-  // S^T of half hf of tile t
-  auto scores = [&](f32x16_t* d, int t, int hf) {
-    const unsigned char* base = smem + (t & 1) * S::TB;
+  auto read_k = [&](int t, int hf, int x) {
     const int row = 32 * hf + kperm;
+    return *(const bf16x8*)(smem + (t & 1) * S::TB + row * S::KROW +
+                            16 * swz<S::KROW>(row, 2 * x + hh));
+  };
+  auto read_v = [&](int t, int hf, int r) {
+    const int d = 32 * (F8 ? r : 2 * (r >> 2) + (r & 1)) + qi;
+    const int ch = F8 ? 2 * hf + hh : 4 * hf + 2 * ((r >> 1) & 1) + hh;
+    return *(const bf16x8*)(smem + (2 + (t & 1)) * S::TB + d * S::VROW + 16 * swz<S::VROW>(d, ch));
+  };
+  // step j of the output (block pair, step u, block, row group) from the
+  // ring, and of the scores
+  constexpr int NO = 2 * S::NDB * NR, NC = S::NS * NR;
+  auto out_step = [&](auto jc, const bf16x8* ring, const bf16x8 (*pr)[2]) {
+    constexpr int j = decltype(jc)::value;
+    constexpr int n = j % NR, x = j / NR, pair = x >> 2, u = (x >> 1) & 1, db = 2 * pair + (x & 1);
+    const bf16x8& f = ring[(F8 ? db : x) % kRing];
+    if constexpr (F8)
+      o[n][db] = mfma32x32x16(e4m3x8_to_bf16(f.w[2 * u], f.w[2 * u + 1]), pr[n][u], o[n][db]);
+    else
+      o[n][db] = mfma32x32x16(f, pr[n][u], o[n][db]);
+  };
+  auto score_step = [&](auto jc, const bf16x8* ring, f32x16_t* d) {
+    constexpr int j = decltype(jc)::value;
+    constexpr int n = j % NR, x = j / NR, r = NVR + (F8 ? x / 2 : x);
+    const bf16x8& f = ring[r % kRing];
+    if constexpr (F8)
+      d[n] = mfma32x32x16(e4m3x8_to_bf16(f.w[2 * (x & 1)], f.w[2 * (x & 1) + 1]), qf[n][x], d[n]);
+    else
+      d[n] = mfma32x32x16(f, qf[n][x], d[n]);
+  };
+  auto clear_scores = [&](f32x16_t* d) {
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
       for (int e = 0; e < 16; ++e) d[n][e] = 0.f;
-    if constexpr (F8) {
-#pragma unroll
-      for (int x = 0; x < S::NS / 2; ++x) {
-        const bf16x8 kk = *(const bf16x8*)(base + row * S::KROW + 16 * swz<S::KROW>(row, 2 * x + hh));
-        const bf16x8 a = e4m3x8_to_bf16(kk.w[0], kk.w[1]), c = e4m3x8_to_bf16(kk.w[2], kk.w[3]);
-#pragma unroll
-        for (int n = 0; n < NR; ++n) d[n] = mfma32x32x16(a, qf[n][2 * x], d[n]);
-#pragma unroll
-        for (int n = 0; n < NR; ++n) d[n] = mfma32x32x16(c, qf[n][2 * x + 1], d[n]);
-      }
-    } else {
-#pragma unroll
-      for (int x = 0; x < S::NS; ++x) {
-        const bf16x8 a = *(const bf16x8*)(base + row * S::KROW + 16 * swz<S::KROW>(row, 2 * x + hh));
-#pragma unroll
-        for (int n = 0; n < NR; ++n) d[n] = mfma32x32x16(a, qf[n][x], d[n]);
-      }
-    }
   };
-  // O^T += V^T P^T of half hf of tile t
-  auto output = [&](int t, int hf) {
-    const unsigned char* base = smem + (2 + (t & 1)) * S::TB;
-    if constexpr (F8) {
-#pragma unroll
-      for (int db = 0; db < S::NDB; ++db) {
-        const int d = 32 * db + qi;
-        const bf16x8 vv = *(const bf16x8*)(base + d * S::VROW + 16 * swz<S::VROW>(d, 2 * hf + hh));
-        const bf16x8 a = e4m3x8_to_bf16(vv.w[0], vv.w[1]), c = e4m3x8_to_bf16(vv.w[2], vv.w[3]);
-#pragma unroll
-        for (int n = 0; n < NR; ++n) o[n][db] = mfma32x32x16(a, pt[n][0], o[n][db]);
-#pragma unroll
-        for (int n = 0; n < NR; ++n) o[n][db] = mfma32x32x16(c, pt[n][1], o[n][db]);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int db = 0; db < S::NDB; ++db) {
-          const int d = 32 * db + qi;
-          const bf16x8 a =
-              *(const bf16x8*)(base + d * S::VROW + 16 * swz<S::VROW>(d, 4 * hf + 2 * u + hh));
-#pragma unroll
-          for (int n = 0; n < NR; ++n) o[n][db] = mfma32x32x16(a, pt[n][u], o[n][db]);
-        }
-    }
+  auto capped = [&](float x) {  // in exponents of 2, of a score
+    return cap - 2.f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * sc) + 1.f);
   };
-  // Half hf of tile t: scores in sa[hf]; the next half's scores go to
-  // sa[hf ^ 1], the previous half's probabilities are in pt.
-  auto half = [&](int t, auto hfc, bool missing) {
+
+  // Half hf of tile t: its scores are in sa[hf].  Output of the half before
+  // (probabilities pt[hf ^ 1]) and scores of the next one (to sa[hf ^ 1]).
+  // The first half of the output's products runs over the maximum of the
+  // scores, the others and the next scores' over the exponentials.
+  auto half = [&](int t, auto hfc) {
     constexpr int hf = decltype(hfc)::value;
     f32x16_t* sv = sa[hf];
+    f32x16_t* sn = sa[hf ^ 1];
+    const bf16x8 (*pr)[2] = pt[hf ^ 1];
+    const int tv = hf ? t : t - 1, tk = hf ? t + 1 : t;
+    bf16x8 ring[kRing];
+    auto read = [&](auto rc) {
+      constexpr int r = decltype(rc)::value;
+      if constexpr (r < NVR) ring[r % kRing] = read_v(tv, hf ^ 1, r);
+      else if constexpr (r < NVR + NKR) ring[r % kRing] = read_k(tk, hf ^ 1, r - NVR);
+    };
+    static_for<0, kAhead>([&](auto rc) { read(rc); });
+
     const int k0 = t * kProTile + 32 * hf;
-    const bool edge = k0 < lo_max || k0 + 32 > hi_min || missing;
-    if (edge) {
+    if (k0 < lo_max || k0 + 32 > hi_min || missing) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int key = k0 + (F8 ? 16 * hh + e : 16 * (e >> 3) + 8 * hh + (e & 7));
-        const bool gone = missing && sPid[(key >> lg) - pg0] < 0;
+        const bool gone = missing && page_of(key) < 0;
 #pragma unroll
         for (int n = 0; n < NR; ++n)
           if (key < lo[n] || key >= hi[n] || gone) sv[n][e] = -INFINITY;
       }
     }
-    float mb[NR];
+
+    // reads per product step: NR steps use one (e4m3: two times NR)
+    constexpr int RS = F8 ? 2 * NR : NR;
+    constexpr int JA = NO / 2, JB = NO - JA + NC, NE = 16 * NR;
+    float mx[NR];
+    static_for<0, JA>([&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      // a pair of blocks is read before its first e4m3 step: same count
+      if constexpr (j % RS == 0) read(IntC<kAhead + j / RS>{});
+      out_step(jc, ring, pr);
+      static_for<NE * j / JA, NE * (j + 1) / JA>([&](auto qc) {
+        constexpr int q = decltype(qc)::value, n = q / 16, e = q % 16;
+        mx[n] = e == 0 ? sv[n][0] : fmaxf(mx[n], sv[n][e]);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
     bool up = false;
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      float m = sv[n][0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) m = fmaxf(m, sv[n][e]);
-      m = half_pair_max(m) * sc;
-      if (CAP)
-        m = m == -INFINITY ? m : cap - 2.f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(m) + 1.f);
-      mb[n] = m;
-      up = up || m > ref[n] + kSlack;
+      float m = half_pair_max(mx[n]);
+      mx[n] = m == -INFINITY ? m : (CAP ? capped(m) : m * sc);
+      up = up || mx[n] > ref[n] + kSlack;
     }
     if (__any(up)) {
       // the probabilities not yet in the output follow it to the new
       // reference (a second rounding to bf16, on the halves where it rises)
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        const float nr = fmaxf(ref[n], mb[n]);
+        const float nr = fmaxf(ref[n], mx[n]);
         const float f = ref[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref[n] - nr);
         ref[n] = nr;
         l_run[n] *= f;
 #pragma unroll
-        for (int db = 0; db < S::NDB; ++db)
+        for (int db = 0; db < S::NDB; ++db) {
+          // (the accumulators stay where they are until here: no copies for
+          // this rare path in the common one)
+          if constexpr (D > 64) asm volatile("" : "+a"(o[n][db]));
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[n][db][e] *= f;
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           float x[8];
-          unpack8(pt[n][u], x);
+          unpack8(pt[hf ^ 1][n][u], x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= f;
-          pt[n][u] = pack8(x);
+          pt[hf ^ 1][n][u] = pack8(x);
         }
       }
     }
-    output(hf ? t : t - 1, hf ^ 1);
-    scores(sa[hf ^ 1], hf ? t + 1 : t, hf ^ 1);
+    float nm[NR], even = 0.f;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const float nm = ref[n] == -INFINITY ? 0.f : -ref[n];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float pv[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = sv[n][8 * u + e];
-          if (CAP) {
-            const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * sc) + 1.f);
-            pv[e] = __builtin_amdgcn_exp2f(fmaf(-2.f * cap, r, cap + nm));
-            if (x == -INFINITY) pv[e] = 0.f;
-          } else {
-            pv[e] = __builtin_amdgcn_exp2f(fmaf(x, sc, nm));
-          }
-          l_run[n] += pv[e];
+    for (int n = 0; n < NR; ++n) nm[n] = ref[n] == -INFINITY ? 0.f : -ref[n];
+    clear_scores(sn);
+    static_for<0, JB>([&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      if constexpr ((JA + j) % RS == 0) read(IntC<kAhead + (JA + j) / RS>{});
+      if constexpr (j < NO - JA) out_step(IntC<JA + j>{}, ring, pr);
+      else score_step(IntC<j - (NO - JA)>{}, ring, sn);
+      static_for<NE * j / JB, NE * (j + 1) / JB>([&](auto qc) {
+        constexpr int q = decltype(qc)::value, n = q / 16, e = q % 16;
+        const float x = sv[n][e];
+        float pv;
+        if constexpr (CAP) {
+          const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * sc) + 1.f);
+          pv = __builtin_amdgcn_exp2f(fmaf(-2.f * cap, r, cap + nm[n]));
+          pv = x == -INFINITY ? 0.f : pv;
+        } else {
+          pv = __builtin_amdgcn_exp2f(fmaf(x, sc, nm[n]));
         }
-        pt[n][u] = pack8(pv);
-      }
-    }
+        if constexpr (e % 2 == 0) {
+          even = pv;
+        } else {
+          uint32_t w2 = f2bf2(even, pv);
+          asm volatile("" : "+v"(w2));  // here, under the products, not behind them
+          pt[hf][n][e >> 3].w[(e & 7) >> 1] = w2;
+          l_run[n] = add_pair(w2, l_run[n]);
+        }
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
 
-  const int CT = kProPages * 16 / kProTile;  // tiles per walk (pages hold 16 tokens or more)
-  for (int c0 = t0; c0 < t1; c0 += CT) {
-    const int c1 = c0 + CT < t1 ? c0 + CT : t1;
-    pg0 = (int)(((int64_t)c0 * kProTile) >> lg);
-    const int pg1 = (int)(((int64_t)c1 * kProTile - 1) >> lg);
+  if (t0 < t1) {
+    // runs begin at whole runs, and so at whole pages (of up to 1024 tokens)
+    const int run0 = t0 & ~(kProRun - 1);
+    if (tid == 0) sMissing = 0;
     __syncthreads();
-    for (int i = tid; i <= pg1 - pg0; i += 256) sPid[i] = paged_page(p.b, b, pg0 + i);
+    fill_ids(run0);
+    fill_ids(run0 + kProRun);
     // the first half's "previous" values: zeros (with zero probabilities)
     for (int i = tid; i < S::TB / 16; i += 256)
-      *(bf16x8*)(smem + (2 + ((c0 + 1) & 1)) * S::TB + 16 * i) = zero8();
+      *(bf16x8*)(smem + (2 + ((t0 + 1) & 1)) * S::TB + 16 * i) = zero8();
 #pragma unroll
-    for (int n = 0; n < NR; ++n) pt[n][0] = pt[n][1] = zero8();
+    for (int n = 0; n < NR; ++n) pt[1][n][0] = pt[1][n][1] = zero8();
     __syncthreads();
-    load_k(c0);
-    wait_vmcnt<0>();
-    __syncthreads();
-    if (c0 + 1 < c1) load_k(c0 + 1);
-    load_v(c0);
-    if (active) scores(sa[0], c0, 0);
-    for (int t = c0; t < c1; ++t) {
-      const bool missing = missing_page(t);
-      if (active) half(t, IntC<0>{}, missing);
-      wait_vmcnt<0>();
-      clear_v(t, missing);
-      // everyone's keys of tile t + 1 and values of tile t are there, and
-      // the keys of tile t and the values of tile t - 1 have been used
-      __syncthreads();
-      if (t + 2 < c1) load_k(t + 2);
-      if (t + 1 < c1) load_v(t + 1);
-      if (active) half(t, IntC<1>{}, missing);
+    {
+      const Ids d = fetch_ids(t0, t0);
+      load_k(t0, d);
+      load_v(t0, d);
     }
-    if (active) output(c1 - 1, 1);
+    wait_vmcnt<LPW>();
+    __syncthreads();  // everyone's first keys
+    if (t0 + 1 < t1) load_k(t0 + 1, fetch_ids(t0 + 1, t0));
+
+    // what a wave does at the turn of tile t: everyone's keys of tile t + 1
+    // and values of tile t are there behind the barrier, and the keys of tile
+    // t and the values of tile t - 1 have been used
+    auto turn = [&](int t, const Ids& d) {
+      wait_vmcnt<0>();
+      clear_v(t);
+      if ((t & (kProRun - 1)) == 2 && t - 2 > run0) fill_ids(t - 2 + kProRun);
+      __syncthreads();
+      if (t + 2 < t1) load_k(t + 2, d);
+      if (t + 1 < t1) load_v(t + 1, d);
+    };
+    if (!active) {  // no rows: this wave only loads
+      for (int t = t0; t < t1; ++t) {
+        missing = sMissing != 0;
+        turn(t, fetch_ids(t + 2, t + 1));
+      }
+    } else {
+      clear_scores(sa[0]);
+      bf16x8 ring[kRing];
+      static_for<0, NKR>([&](auto xc) {
+        constexpr int x = decltype(xc)::value, r = NVR + x;
+        ring[r % kRing] = read_k(t0, 0, x);
+        static_for<0, F8 ? 2 * NR : NR>(
+            [&](auto nc) { score_step(IntC<(F8 ? 2 * NR : NR) * x + decltype(nc)::value>{}, ring, sa[0]); });
+      });
+      for (int t = t0; t < t1; ++t) {
+        missing = __builtin_amdgcn_readfirstlane(sMissing) != 0;
+        const Ids d = fetch_ids(t + 2, t + 1);
+        half(t, IntC<0>{});
+        turn(t, d);
+        half(t, IntC<1>{});
+      }
+      static_for<0, kRing>([&](auto rc) {
+        constexpr int r = decltype(rc)::value;
+        if constexpr (r < NVR) ring[r] = read_v(t1 - 1, 1, r);
+      });
+      static_assert(!F8 || NVR <= kRing, "e4m3 blocks fit the ring");
+      static_for<0, NO>([&](auto jc) {
+        constexpr int j = decltype(jc)::value, r = j / NR;
+        out_step(jc, ring, pt[1]);
+        // the last use of a value read makes room for the next one
+        if constexpr (!F8 && j % NR == NR - 1 && r + kRing < NVR)
+          ring[r % kRing] = read_v(t1 - 1, 1, r + kRing);
+      });
+    }
   }
 
   if (!active && p.splits == 1) return;
