@@ -564,6 +564,37 @@ __device__ __forceinline__ float add_pair(uint32_t w, float l) {
                                          __builtin_bit_cast(bf16x2_t, 0x3f803f80u), l, false);
 }
 
+// The products with their operands where the kernel wants them: scores in
+// vector registers, which the exponentials read; output and queries in
+// accumulation registers, which nothing else reads in the common path.  (The
+// compiler would copy scores or output from one file to the other in every
+// half: 3.4 us a tile of 64 keys and 256 rows of 128 dims.)  It does not know
+// when these products finish: what reads their results must come 20 wait
+// states or more behind the last one (mfma_settle).  NOP: the operand of the
+// vector registers is just computed, which needs two wait states.
+template <bool FIRST, bool NOP>
+__device__ __forceinline__ void mfma_scores(f32x16_t& d, const bf16x8& k, const bf16x8& q) {
+  const i32x4_t a = __builtin_bit_cast(i32x4_t, k), c = __builtin_bit_cast(i32x4_t, q);
+  if constexpr (FIRST && NOP)
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(c));
+  else if constexpr (FIRST)
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(d) : "v"(a), "a"(c));
+  else if constexpr (NOP)
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "a"(c));
+  else
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "a"(c));
+}
+
+template <bool NOP>
+__device__ __forceinline__ void mfma_output(f32x16_t& d, const bf16x8& v, const bf16x8& pr) {
+  const i32x4_t a = __builtin_bit_cast(i32x4_t, v), c = __builtin_bit_cast(i32x4_t, pr);
+  if constexpr (NOP)
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(d) : "v"(a), "v"(c));
+  else
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(d) : "v"(a), "v"(c));
+}
+__device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 15"); }
+
 template <int D, bool F8>
 struct ProShape {
   static constexpr int NR = D == 256 ? 1 : 2;   // 32-row groups per wave
@@ -575,6 +606,34 @@ struct ProShape {
   static constexpr int NDB = D / 32;            // output blocks
   static constexpr int NS = D / 16;             // MFMA steps of a score
   static constexpr int PF = BM * (D + 2);       // floats of a partial
+
+  // Products of a half: JA steps of the output, the scores' NC, the rest of
+  // the output's NO.  Their operand fragments come from LDS in that order,
+  // through a ring of registers, read kAhead fragments before their product.
+  // An output step is (block pair, step u, block, row group); e4m3 fragments
+  // hold both steps u of a block, or two steps of the scores.
+  static constexpr int NVR = F8 ? NDB : 2 * NDB;  // fragments of values
+  static constexpr int NKR = F8 ? NS / 2 : NS;    // fragments of keys
+  static constexpr int NO = 2 * NDB * NR, NC = NS * NR, JA = NO / 2;
+  static constexpr int NVA = F8 && D == 64 ? NVR : NVR / 2;  // values' that the first JA use
+  static constexpr int kRing = D == 64 ? 4 : 8, kAhead = D == 64 ? 3 : 6;
+  // the output's fragment of its step j
+  static constexpr int out_frag(int j) {
+    const int x = j / NR;
+    return F8 ? 2 * (x >> 2) + (x & 1) : x;
+  }
+  // the fragment, in reading order, of step j of a half
+  static constexpr int frag_at(int j) {
+    if (j >= JA && j < JA + NC) return NVA + (j - JA) / NR / (F8 ? 2 : 1);
+    const int r = out_frag(j < JA ? j : j - NC);
+    return r < NVA ? r : r + NKR;
+  }
+  // fragments read by the start of step j's product
+  static constexpr int frags_to(int j) {
+    int m = 0;
+    for (int i = 0; i <= j; ++i) m = frag_at(i) + 1 > m ? frag_at(i) + 1 : m;
+    return m;
+  }
 };
 
 // 16-byte slot of logical chunk c of LDS row `row` (RB bytes long): rows that
@@ -637,7 +696,7 @@ __device__ bool find_tile(const PagedAttn& p, int item, int64_t* scan, int* foun
 }
 
 template <int D, bool F8, bool CAP>
-__global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(PagedAttn p) {
+__global__ __launch_bounds__(256, 1) void paged_prompt_kernel(PagedAttn p) {
   using S = ProShape<D, F8>;
   constexpr int NR = S::NR;
   __shared__ __align__(16) unsigned char smem[4 * S::TB];
@@ -824,13 +883,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
     }
   };
 
-  // Operand fragments of a half, in the order of their products: output block
-  // pairs (bf16: steps u of both blocks; e4m3: both steps of a block in one
-  // read), then the scores' steps.  They go through a ring of registers, read
-  // kAhead before their products.
-  constexpr int NVR = F8 ? S::NDB : 2 * S::NDB;  // reads of values
-  constexpr int NKR = F8 ? S::NS / 2 : S::NS;    // reads of keys
-  constexpr int kRing = D == 64 ? 4 : 8, kAhead = D == 64 ? 3 : 6;
+  constexpr int NVR = S::NVR, NKR = S::NKR, NVA = S::NVA, NO = S::NO, NC = S::NC, JA = S::JA;
+  constexpr int kRing = S::kRing, kAhead = S::kAhead;
   const int kperm = F8 ? 16 * ((qi >> 2) & 1) + 8 * (qi >> 4) + 4 * ((qi >> 3) & 1) + (qi & 3)
                        : 16 * (qi >> 4) + 8 * ((qi >> 2) & 1) + 4 * ((qi >> 3) & 1) + (qi & 3);
   auto read_k = [&](int t, int hf, int x) {
@@ -843,79 +897,69 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
     const int ch = F8 ? 2 * hf + hh : 4 * hf + 2 * ((r >> 1) & 1) + hh;
     return *(const bf16x8*)(smem + (2 + (t & 1)) * S::TB + d * S::VROW + 16 * swz<S::VROW>(d, ch));
   };
-  // step j of the output (block pair, step u, block, row group) from the
-  // ring, and of the scores
-  constexpr int NO = 2 * S::NDB * NR, NC = S::NS * NR;
-  auto out_step = [&](auto jc, const bf16x8* ring, const bf16x8 (*pr)[2]) {
+  auto out_step = [&](auto jc, const bf16x8& f, const bf16x8 (*pr)[2]) {
     constexpr int j = decltype(jc)::value;
     constexpr int n = j % NR, x = j / NR, pair = x >> 2, u = (x >> 1) & 1, db = 2 * pair + (x & 1);
-    const bf16x8& f = ring[(F8 ? db : x) % kRing];
     if constexpr (F8)
-      o[n][db] = mfma32x32x16(e4m3x8_to_bf16(f.w[2 * u], f.w[2 * u + 1]), pr[n][u], o[n][db]);
+      mfma_output<true>(o[n][db], e4m3x8_to_bf16(f.w[2 * u], f.w[2 * u + 1]), pr[n][u]);
     else
-      o[n][db] = mfma32x32x16(f, pr[n][u], o[n][db]);
+      mfma_output<false>(o[n][db], f, pr[n][u]);
   };
-  auto score_step = [&](auto jc, const bf16x8* ring, f32x16_t* d) {
-    constexpr int j = decltype(jc)::value;
-    constexpr int n = j % NR, x = j / NR, r = NVR + (F8 ? x / 2 : x);
-    const bf16x8& f = ring[r % kRing];
+  auto score_step = [&](auto jc, const bf16x8& f, f32x16_t* d) {
+    constexpr int j = decltype(jc)::value, n = j % NR, x = j / NR;
     if constexpr (F8)
-      d[n] = mfma32x32x16(e4m3x8_to_bf16(f.w[2 * (x & 1)], f.w[2 * (x & 1) + 1]), qf[n][x], d[n]);
+      mfma_scores<x == 0, true>(d[n], e4m3x8_to_bf16(f.w[2 * (x & 1)], f.w[2 * (x & 1) + 1]), qf[n][x]);
     else
-      d[n] = mfma32x32x16(f, qf[n][x], d[n]);
-  };
-  auto clear_scores = [&](f32x16_t* d) {
-#pragma unroll
-    for (int n = 0; n < NR; ++n)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) d[n][e] = 0.f;
+      mfma_scores<x == 0, false>(d[n], f, qf[n][x]);
   };
   auto capped = [&](float x) {  // in exponents of 2, of a score
     return cap - 2.f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * sc) + 1.f);
   };
+  auto seen = [&](int key, int n) {
+    return key >= lo[n] && key < hi[n] && !(missing && page_of(key) < 0);
+  };
+  // key of element e of a half's scores, from the half's first
+  auto key_at = [&](int e) { return F8 ? 16 * hh + e : 16 * (e >> 3) + 8 * hh + (e & 7); };
 
   // Half hf of tile t: its scores are in sa[hf].  Output of the half before
-  // (probabilities pt[hf ^ 1]) and scores of the next one (to sa[hf ^ 1]).
-  // The first half of the output's products runs over the maximum of the
-  // scores, the others and the next scores' over the exponentials.
+  // (probabilities pt[hf ^ 1], which also enter the row sums here) and scores
+  // of the next one (to sa[hf ^ 1]).  The first JA products run over the
+  // maximum of the scores, the others over the exponentials.
   auto half = [&](int t, auto hfc) {
     constexpr int hf = decltype(hfc)::value;
     f32x16_t* sv = sa[hf];
     f32x16_t* sn = sa[hf ^ 1];
-    const bf16x8 (*pr)[2] = pt[hf ^ 1];
+    bf16x8 (*pr)[2] = pt[hf ^ 1];
     const int tv = hf ? t : t - 1, tk = hf ? t + 1 : t;
     bf16x8 ring[kRing];
     auto read = [&](auto rc) {
       constexpr int r = decltype(rc)::value;
-      if constexpr (r < NVR) ring[r % kRing] = read_v(tv, hf ^ 1, r);
-      else if constexpr (r < NVR + NKR) ring[r % kRing] = read_k(tk, hf ^ 1, r - NVR);
+      if constexpr (r < NVA) ring[r % kRing] = read_v(tv, hf ^ 1, r);
+      else if constexpr (r < NVA + NKR) ring[r % kRing] = read_k(tk, hf ^ 1, r - NVA);
+      else if constexpr (r < NVR + NKR) ring[r % kRing] = read_v(tv, hf ^ 1, r - NKR);
     };
     static_for<0, kAhead>([&](auto rc) { read(rc); });
 
     const int k0 = t * kProTile + 32 * hf;
-    if (k0 < lo_max || k0 + 32 > hi_min || missing) {
+    const bool edge = k0 < lo_max || k0 + 32 > hi_min || missing;
+    if (edge) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int key = k0 + (F8 ? 16 * hh + e : 16 * (e >> 3) + 8 * hh + (e & 7));
-        const bool gone = missing && page_of(key) < 0;
+      for (int e = 0; e < 16; ++e)
 #pragma unroll
         for (int n = 0; n < NR; ++n)
-          if (key < lo[n] || key >= hi[n] || gone) sv[n][e] = -INFINITY;
-      }
+          if (!seen(k0 + key_at(e), n)) sv[n][e] = -INFINITY;
     }
 
-    // reads per product step: NR steps use one (e4m3: two times NR)
-    constexpr int RS = F8 ? 2 * NR : NR;
-    constexpr int JA = NO / 2, JB = NO - JA + NC, NE = 16 * NR;
+    constexpr int JB = NO - JA + NC, NE = 16 * NR;
     float mx[NR];
     static_for<0, JA>([&](auto jc) {
       constexpr int j = decltype(jc)::value;
-      // a pair of blocks is read before its first e4m3 step: same count
-      if constexpr (j % RS == 0) read(IntC<kAhead + j / RS>{});
-      out_step(jc, ring, pr);
+      static_for<j ? kAhead + S::frags_to(j - 1) : kAhead, kAhead + S::frags_to(j)>([&](auto rc) { read(rc); });
+      out_step(jc, ring[S::frag_at(j) % kRing], pr);
       static_for<NE * j / JA, NE * (j + 1) / JA>([&](auto qc) {
         constexpr int q = decltype(qc)::value, n = q / 16, e = q % 16;
         mx[n] = e == 0 ? sv[n][0] : fmaxf(mx[n], sv[n][e]);
+        if constexpr (e % 2 == 1) l_run[n] = add_pair(pr[n][e >> 3].w[(e & 7) >> 1], l_run[n]);
       });
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -929,6 +973,7 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
     if (__any(up)) {
       // the probabilities not yet in the output follow it to the new
       // reference (a second rounding to bf16, on the halves where it rises)
+      mfma_settle();
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         const float nr = fmaxf(ref[n], mx[n]);
@@ -937,39 +982,37 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
         l_run[n] *= f;
 #pragma unroll
         for (int db = 0; db < S::NDB; ++db) {
-          // (the accumulators stay where they are until here: no copies for
-          // this rare path in the common one)
-          if constexpr (D > 64) asm volatile("" : "+a"(o[n][db]));
+          asm volatile("" : "+a"(o[n][db]));  // not copied before it is settled
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[n][db][e] *= f;
+          asm volatile("" : "+a"(o[n][db]));  // and back before the paths join
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           float x[8];
-          unpack8(pt[hf ^ 1][n][u], x);
+          unpack8(pr[n][u], x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] *= f;
-          pt[hf ^ 1][n][u] = pack8(x);
+          pr[n][u] = pack8(x);
         }
       }
     }
     float nm[NR], even = 0.f;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) nm[n] = ref[n] == -INFINITY ? 0.f : -ref[n];
-    clear_scores(sn);
+    for (int n = 0; n < NR; ++n) nm[n] = (CAP ? cap : 0.f) - (ref[n] == -INFINITY ? 0.f : ref[n]);
     static_for<0, JB>([&](auto jc) {
-      constexpr int j = decltype(jc)::value;
-      if constexpr ((JA + j) % RS == 0) read(IntC<kAhead + (JA + j) / RS>{});
-      if constexpr (j < NO - JA) out_step(IntC<JA + j>{}, ring, pr);
-      else score_step(IntC<j - (NO - JA)>{}, ring, sn);
-      static_for<NE * j / JB, NE * (j + 1) / JB>([&](auto qc) {
+      constexpr int j = JA + decltype(jc)::value, jb = decltype(jc)::value;
+      static_for<kAhead + S::frags_to(j - 1), kAhead + S::frags_to(j)>([&](auto rc) { read(rc); });
+      const bf16x8& f = ring[S::frag_at(j) % kRing];
+      if constexpr (jb < NC) score_step(IntC<jb>{}, f, sn);
+      else out_step(IntC<j - NC>{}, f, pr);
+      static_for<NE * jb / JB, NE * (jb + 1) / JB>([&](auto qc) {
         constexpr int q = decltype(qc)::value, n = q / 16, e = q % 16;
         const float x = sv[n][e];
         float pv;
         if constexpr (CAP) {
           const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * sc) + 1.f);
-          pv = __builtin_amdgcn_exp2f(fmaf(-2.f * cap, r, cap + nm[n]));
-          pv = x == -INFINITY ? 0.f : pv;
+          pv = __builtin_amdgcn_exp2f(fmaf(-2.f * cap, r, nm[n]));
         } else {
           pv = __builtin_amdgcn_exp2f(fmaf(x, sc, nm[n]));
         }
@@ -979,11 +1022,18 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
           uint32_t w2 = f2bf2(even, pv);
           asm volatile("" : "+v"(w2));  // here, under the products, not behind them
           pt[hf][n][e >> 3].w[(e & 7) >> 1] = w2;
-          l_run[n] = add_pair(w2, l_run[n]);
         }
       });
       __builtin_amdgcn_sched_barrier(0);
     });
+    // (a capped score of minus infinity is minus the cap)
+    if (CAP && edge) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+          if (!seen(k0 + key_at(e), n)) pt[hf][n][e >> 3].w[(e & 7) >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
+    }
   };
 
   if (t0 < t1) {
@@ -1025,14 +1075,11 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
         turn(t, fetch_ids(t + 2, t + 1));
       }
     } else {
-      clear_scores(sa[0]);
-      bf16x8 ring[kRing];
-      static_for<0, NKR>([&](auto xc) {
-        constexpr int x = decltype(xc)::value, r = NVR + x;
-        ring[r % kRing] = read_k(t0, 0, x);
-        static_for<0, F8 ? 2 * NR : NR>(
-            [&](auto nc) { score_step(IntC<(F8 ? 2 * NR : NR) * x + decltype(nc)::value>{}, ring, sa[0]); });
+      static_for<0, NC>([&](auto jc) {
+        constexpr int j = decltype(jc)::value;
+        score_step(jc, read_k(t0, 0, j / (F8 ? 2 * NR : NR)), sa[0]);
       });
+      mfma_settle();
       for (int t = t0; t < t1; ++t) {
         missing = __builtin_amdgcn_readfirstlane(sMissing) != 0;
         const Ids d = fetch_ids(t + 2, t + 1);
@@ -1040,18 +1087,14 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
         turn(t, d);
         half(t, IntC<1>{});
       }
-      static_for<0, kRing>([&](auto rc) {
-        constexpr int r = decltype(rc)::value;
-        if constexpr (r < NVR) ring[r] = read_v(t1 - 1, 1, r);
-      });
-      static_assert(!F8 || NVR <= kRing, "e4m3 blocks fit the ring");
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) l_run[n] = add_pair(pt[1][n][e >> 2].w[e & 3], l_run[n]);
       static_for<0, NO>([&](auto jc) {
-        constexpr int j = decltype(jc)::value, r = j / NR;
-        out_step(jc, ring, pt[1]);
-        // the last use of a value read makes room for the next one
-        if constexpr (!F8 && j % NR == NR - 1 && r + kRing < NVR)
-          ring[r % kRing] = read_v(t1 - 1, 1, r + kRing);
+        out_step(jc, read_v(t1 - 1, 1, S::out_frag(decltype(jc)::value)), pt[1]);
       });
+      mfma_settle();
     }
   }
 
@@ -1068,6 +1111,8 @@ __global__ __launch_bounds__(256, D == 64 ? 2 : 1) void paged_prompt_kernel(Page
   for (int n = 0; n < NR; ++n) {
     const int i = 32 * NR * w + 32 * n + qi;
     const float l = half_pair_sum(l_run[n]);
+#pragma unroll
+    for (int db = 0; db < S::NDB; ++db) asm volatile("" : "+a"(o[n][db]));
     if (i >= rows) continue;
     if (p.splits == 1) {
       const float inv = l > 0.f ? vs / l : 0.f;
