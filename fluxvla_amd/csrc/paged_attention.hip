@@ -597,7 +597,7 @@ __device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 
 
 template <int D, bool F8>
 struct ProShape {
-  static constexpr int NR = D == 256 ? 1 : 2;   // 32-row groups per wave
+  static constexpr int NR = 1;   // 32-row groups per wave
   static constexpr int BM = 128 * NR;           // rows per workgroup
   static constexpr int ES = F8 ? 1 : 2;
   static constexpr int KROW = D * ES;           // bytes of a key in LDS
@@ -696,7 +696,7 @@ __device__ bool find_tile(const PagedAttn& p, int item, int64_t* scan, int* foun
 }
 
 template <int D, bool F8, bool CAP>
-__global__ __launch_bounds__(256, 1) void paged_prompt_kernel(PagedAttn p) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(PagedAttn p) {
   using S = ProShape<D, F8>;
   constexpr int NR = S::NR;
   __shared__ __align__(16) unsigned char smem[4 * S::TB];
@@ -1211,7 +1211,7 @@ static PagedPlan paged_plan(const fvx_paged_attn_desc* d) {
   a.prec = a.part + (int64_t)a.n_wg * 2 * kDecRows * (d->head_dim + 2) * 4;
   a.ppart = a.bytes = a.prec;
   if (a.many) {
-    const int64_t bm = d->head_dim == 256 ? 128 : 256;
+    const int64_t bm = 128;
     a.problems = (d->n_rows * G / bm + (d->n_seqs < d->n_rows ? d->n_seqs : d->n_rows)) * d->kv_heads;
     // one workgroup per CU: with fewer problems their keys are split
     const int64_t s = device_cus() / a.problems;
