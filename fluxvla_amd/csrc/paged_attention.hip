@@ -542,20 +542,28 @@ constexpr int kProRun = 128;
 constexpr int kProPages = 2 * kProRun * kProTile / 16;
 constexpr float kSlack = 8.f;
 
-// 16 bytes per lane from 64-bit addresses, or from a uniform base and 32-bit
-// offsets, straight into LDS (lane l's at lds + 16 l); waited for with
-// wait_vmcnt, like load_lds16.
+// 16 bytes per lane straight into LDS (lane l's at m0 + OFF + 16 l), from
+// 64-bit addresses or from a uniform base and 32-bit offsets (+ OFF); waited
+// for with wait_vmcnt, like load_lds16.
 __device__ __forceinline__ void load_lds16_at(const void* a, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off"
                :
                : "s"(lds), "v"(a)
                : "memory");
 }
+template <int OFF>
 __device__ __forceinline__ void load_lds16_at(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3"
                :
-               : "s"(lds), "v"(off), "s"(base)
+               : "s"(lds), "v"(off), "s"(base), "n"(OFF)
                : "memory");
+}
+
+// max(a, b, c), without the compiler's quieting of each
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 // l + the two bf16 values of w, as the second product reads them.
@@ -781,27 +789,29 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       for (int e = 0; e < 16; ++e) o[n][db][e] = 0.f;
   }
 
-  // DMA: instruction L = LPW w + i (1 KiB) brings K rows RPK L .. or dims RPV L
-  // ... of a tile.  Its K rows share a page.  A tile's values share one when
-  // pages hold a tile or more; otherwise a lane's keys do, at a place in the
-  // page that is the same in every tile.
-  const uint32_t lds = lds_addr(smem);
+  // DMA: a wave brings 16 keys and D / 4 dims of a tile, LPW instructions of
+  // 1 KiB each: RPK keys or RPV dims.  Its keys share a page.  A tile's
+  // values share one when pages hold a tile or more; otherwise a lane's keys
+  // do, at a place in the page that is the same in every tile.
   constexpr int LPW = S::TB / 1024 / 4;
   constexpr int CK = S::KROW / 16, CV = S::VROW / 16, RPK = 64 / CK, RPV = 64 / CV;
   constexpr int NV = LPW > 1 && !F8 ? 2 : 1;  // key chunks that differ over i
+  const uint32_t lds = lds_addr(smem) + 1024 * LPW * w;
   const int mask = (1 << lg) - 1;
   const bool big_page = (1 << lg) >= kProTile;
-  const int64_t head_k = (int64_t)S::KROW << lg, head_v = ((int64_t)D * S::ES) << lg;  // bytes
+  const uint32_t page_bytes = ((uint32_t)p.kv_heads * D * S::ES) << lg;  // at most 2^31
+  const unsigned char* k_head = p.k + (((int64_t)h * D * S::ES) << lg);
+  const unsigned char* v_head = p.v + (((int64_t)h * D * S::ES) << lg);
   uint32_t koff[LPW];
 #pragma unroll
   for (int i = 0; i < LPW; ++i)
-    koff[i] = (lane / CK) * S::KROW + 16 * swz<S::KROW>(RPK * (LPW * w + i) + lane / CK, lane % CK);
+    koff[i] = (lane / CK) * S::KROW + 16 * swz<S::KROW>(16 * w + RPK * i + lane / CK, lane % CK) +
+              1024 * (i & ~3);
   int vchunk[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) vchunk[i] = swz<S::VROW>(RPV * (LPW * w + i) + lane / CV, lane % CV);
   const uint32_t vrow = ((uint32_t)(RPV * LPW * w + lane / CV) * S::ES) << lg;
 
-  bool missing = false;  // has a page so far not existed?
   // the page of a token, -1 for none
   auto page_of = [&](int key) { return sPid[(key >> lg) & (kProPages - 1)]; };
   // ids of the pages of tiles [ta, ta + kProRun), by all threads
@@ -813,49 +823,48 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       if (id < 0 && (int64_t)(first + i) << lg < hi_max) sMissing = 1;
     }
   };
+  bool missing = false;  // has a page so far not existed?
   struct Ids {
-    int k[LPW], v[NV];
+    int k, v[NV], none;
   };
   // page ids for load_k(tk) and load_v(tv), ahead of them
   auto fetch_ids = [&](int tk, int tv) {
     Ids d;
-#pragma unroll
-    for (int i = 0; i < LPW; ++i)
-      d.k[i] = page_of(tk * kProTile + RPK * (LPW * w + i));
+    d.k = page_of(tk * kProTile + 16 * w);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       d.v[i] = page_of(tv * kProTile + (big_page ? 0 : vchunk[i] * (16 / S::ES)));
+    d.none = sMissing;
     return d;
   };
   auto load_k = [&](int t, const Ids& d) {
-#pragma unroll
-    for (int i = 0; i < LPW; ++i) {
-      const int L = LPW * w + i;
-      const int id = __builtin_amdgcn_readfirstlane(d.k[i] < 0 ? 0 : d.k[i]);
-      const int64_t at = ((int64_t)id * p.kv_heads + h) * head_k +
-                         ((t * kProTile + RPK * L) & mask) * S::KROW;
-      load_lds16_at(p.k + at, koff[i], lds + (t & 1) * S::TB + 1024 * L);
-    }
+    const uint32_t id = __builtin_amdgcn_readfirstlane(d.k < 0 ? 0 : d.k);
+    const unsigned char* at =
+        k_head + (uint64_t)id * page_bytes + ((t * kProTile + 16 * w) & mask) * S::KROW;
+    const uint32_t to = lds + (t & 1) * S::TB;
+    static_for<0, LPW>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      load_lds16_at<1024 * (i & 3)>(at, koff[i], to + 1024 * (i & ~3));
+    });
   };
   auto load_v = [&](int t, const Ids& d) {
+    const uint32_t to = lds + (2 + (t & 1)) * S::TB;
     if (big_page) {
-      const int id = __builtin_amdgcn_readfirstlane(d.v[0] < 0 ? 0 : d.v[0]);
-      const unsigned char* at = p.v + ((int64_t)id * p.kv_heads + h) * head_v +
-                                ((t * kProTile) & mask) * S::ES;
+      const uint32_t id = __builtin_amdgcn_readfirstlane(d.v[0] < 0 ? 0 : d.v[0]);
+      const unsigned char* at = v_head + (uint64_t)id * page_bytes + ((t * kProTile) & mask) * S::ES;
 #pragma unroll
       for (int i = 0; i < LPW; ++i)
-        load_lds16_at(at, vrow + (((uint32_t)i * RPV * S::ES) << lg) + 16 * vchunk[i % NV],
-                      lds + (2 + (t & 1)) * S::TB + 1024 * (LPW * w + i));
+        load_lds16_at<0>(at + (((uint32_t)i * RPV * S::ES) << lg), vrow + 16 * vchunk[i % NV],
+                         to + 1024 * i);
     } else {
       const unsigned char* at[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        at[i] = p.v + ((int64_t)(d.v[i] < 0 ? 0 : d.v[i]) * p.kv_heads + h) * head_v + vrow +
+        at[i] = v_head + (uint64_t)(uint32_t)(d.v[i] < 0 ? 0 : d.v[i]) * page_bytes + vrow +
                 ((vchunk[i] * (16 / S::ES)) & mask) * S::ES;
 #pragma unroll
       for (int i = 0; i < LPW; ++i)
-        load_lds16_at(at[i % NV] + (((uint32_t)i * RPV * S::ES) << lg),
-                      lds + (2 + (t & 1)) * S::TB + 1024 * (LPW * w + i));
+        load_lds16_at(at[i % NV] + (((uint32_t)i * RPV * S::ES) << lg), to + 1024 * i);
     }
   };
   // values that no row of the tile sees (unwritten slots, missing pages) may
@@ -915,9 +924,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   auto capped = [&](float x) {  // in exponents of 2, of a score
     return cap - 2.f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * sc) + 1.f);
   };
-  auto seen = [&](int key, int n) {
-    return key >= lo[n] && key < hi[n] && !(missing && page_of(key) < 0);
-  };
   // key of element e of a half's scores, from the half's first
   auto key_at = [&](int e) { return F8 ? 16 * hh + e : 16 * (e >> 3) + 8 * hh + (e & 7); };
 
@@ -942,12 +948,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
 
     const int k0 = t * kProTile + 32 * hf;
     const bool edge = k0 < lo_max || k0 + 32 > hi_min || missing;
+    // keys of this lane that exist, bit e
+    auto there = [&] {
+      uint32_t m = 0xffffu;
+      if (missing) {
+        m = 0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m |= (page_of(k0 + key_at(e)) < 0 ? 0u : 1u) << e;
+      }
+      return m;
+    };
     if (edge) {
+      const uint32_t ok = there();
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
+      for (int n = 0; n < NR; ++n) {
+        const uint32_t span = (uint32_t)(hi[n] - lo[n]), at = (uint32_t)(k0 - lo[n]);
 #pragma unroll
-        for (int n = 0; n < NR; ++n)
-          if (!seen(k0 + key_at(e), n)) sv[n][e] = -INFINITY;
+        for (int e = 0; e < 16; ++e) {
+          const bool in = (at + (uint32_t)key_at(e) < span) & ((ok >> e & 1) != 0);
+          sv[n][e] = in ? sv[n][e] : -INFINITY;
+        }
+      }
     }
 
     constexpr int JB = NO - JA + NC, NE = 16 * NR;
@@ -958,7 +979,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       out_step(jc, ring[S::frag_at(j) % kRing], pr);
       static_for<NE * j / JA, NE * (j + 1) / JA>([&](auto qc) {
         constexpr int q = decltype(qc)::value, n = q / 16, e = q % 16;
-        mx[n] = e == 0 ? sv[n][0] : fmaxf(mx[n], sv[n][e]);
+        if constexpr (e % 2 == 1) mx[n] = max3(e == 1 ? sv[n][0] : mx[n], sv[n][e - 1], sv[n][e]);
         if constexpr (e % 2 == 1) l_run[n] = add_pair(pr[n][e >> 3].w[(e & 7) >> 1], l_run[n]);
       });
       __builtin_amdgcn_sched_barrier(0);
@@ -1029,10 +1050,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     // (a capped score of minus infinity is minus the cap)
     if (CAP && edge) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int n = 0; n < NR; ++n)
-          if (!seen(k0 + key_at(e), n)) pt[hf][n][e >> 3].w[(e & 7) >> 1] &= e & 1 ? 0xffffu : 0xffff0000u;
+        for (int e = 0; e < 16; ++e)
+          pt[hf][n][e >> 3].w[(e & 7) >> 1] &=
+              sv[n][e] == -INFINITY ? (e & 1 ? 0xffffu : 0xffff0000u) : 0xffffffffu;
     }
   };
 
@@ -1056,7 +1078,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     }
     wait_vmcnt<LPW>();
     __syncthreads();  // everyone's first keys
-    if (t0 + 1 < t1) load_k(t0 + 1, fetch_ids(t0 + 1, t0));
+    {
+      const Ids d = fetch_ids(t0 + 1, t0);
+      missing = __builtin_amdgcn_readfirstlane(d.none) != 0;
+      if (t0 + 1 < t1) load_k(t0 + 1, d);
+    }
 
     // what a wave does at the turn of tile t: everyone's keys of tile t + 1
     // and values of tile t are there behind the barrier, and the keys of tile
@@ -1065,13 +1091,14 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       wait_vmcnt<0>();
       clear_v(t);
       if ((t & (kProRun - 1)) == 2 && t - 2 > run0) fill_ids(t - 2 + kProRun);
+      // (a run's pages are looked up a hundred tiles before they are used)
+      missing = __builtin_amdgcn_readfirstlane(d.none) != 0;
       __syncthreads();
       if (t + 2 < t1) load_k(t + 2, d);
       if (t + 1 < t1) load_v(t + 1, d);
     };
     if (!active) {  // no rows: this wave only loads
       for (int t = t0; t < t1; ++t) {
-        missing = sMissing != 0;
         turn(t, fetch_ids(t + 2, t + 1));
       }
     } else {
@@ -1081,7 +1108,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
       });
       mfma_settle();
       for (int t = t0; t < t1; ++t) {
-        missing = __builtin_amdgcn_readfirstlane(sMissing) != 0;
         const Ids d = fetch_ids(t + 2, t + 1);
         half(t, IntC<0>{});
         turn(t, d);
