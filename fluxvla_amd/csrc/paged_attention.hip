@@ -23,6 +23,22 @@ namespace fvx {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// n / d for n < 2^31 by one multiplication
+struct FastDiv {
+  uint32_t d, mul, shift;
+  static FastDiv of(uint32_t d) {
+    FastDiv f;
+    f.d = d;
+    f.shift = 0;
+    while ((1ull << f.shift) < d) ++f.shift;
+    f.mul = (uint32_t)((((1ull << f.shift) - d) << 32) / d + 1);
+    return f;
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+  }
+};
+
 struct PagedAttn {
   PagedBatch b;
   const bf16_t* q;
@@ -35,6 +51,7 @@ struct PagedAttn {
   const float* v_scale;
   const int32_t* prefix_len;
   int32_t kv_heads, group, window;
+  FastDiv by_group;
   float scale, softcap;
   // few rows: sequences of at most most_rows query rows per key/value head
   int32_t most_rows;
@@ -93,12 +110,14 @@ struct PagedSeq {
 // Few rows per sequence: up to 16 rows a problem on 16x16x32 MFMAs
 // ---------------------------------------------------------------------------
 // Bound by the cache's bytes.  All (sequence, key/value head, 16 rows)
-// problems form one line of units of kUnitBlocks key blocks, which is cut
-// evenly over the workgroups: lengths may differ as they like, and the host
-// need not know them.  A workgroup walks its piece problem by problem, its
-// four waves taking the key blocks in turn; a problem that crosses workgroups
+// problems form one line of units of kWaves key blocks, which is cut evenly
+// over the workgroups, one per CU: lengths may differ as they like, and the
+// host need not know them.  A workgroup walks its piece problem by problem,
+// its waves taking the key blocks in turn; a problem that crosses workgroups
 // leaves fp32 partials (rows, maxima, sums) and the merge kernel adds them in
-// workgroup order.
+// workgroup order.  (With two workgroups of 4 waves per CU the memory serves
+// the older one first: it was done at 145 us of 187 and left the other alone
+// with half the loads in flight.)
 //
 // Key blocks: 32 keys of bf16, 64 of e4m3 -- 16 bytes per lane and load.  Lane
 // (m = l % 16, g = l / 16) reads, for S^T tile t, key GS (m / 4) + 4 t + m % 4
@@ -108,13 +127,14 @@ struct PagedSeq {
 // memory to registers; the next block's keys are requested once S^T has used
 // the current ones, its values once O^T has.
 constexpr int kDecRows = 16;
-constexpr int kUnitBlocks = 4;
+constexpr int kWaves = 8;
 constexpr int kPageIds = 1024;  // page ids of a walk held in LDS
 
 template <int D, bool F8>
 struct DecShape {
   static constexpr int ES = F8 ? 1 : 2;        // bytes per cache value
   static constexpr int KB = F8 ? 64 : 32;      // keys per block
+  static constexpr int UB = KB * kWaves;       // keys per unit
   static constexpr int GS = KB / 4;            // keys per lane group
   static constexpr int NT = KB / 16;           // S^T tiles
   static constexpr int NK = D * ES / 64;       // 16-byte loads per key row
@@ -123,14 +143,40 @@ struct DecShape {
   static constexpr int PF = kDecRows * (D + 2);  // floats of a partial
 };
 
+// a / b for a >= 0, b > 0; almost always in 32 bits
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
+  if ((uint64_t)(a | b) >> 32 == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
+
+// The line of units cut into `parts` pieces as even as they go: the first
+// `more` of them have `each` + 1 units.
+struct Pieces {
+  int64_t each, more;
+  __device__ __forceinline__ Pieces(int64_t total, int parts) {
+    each = div64(total, parts);
+    more = total - each * parts;
+  }
+  __device__ __forceinline__ int64_t start(int w) const {
+    return w * each + (w < more ? w : more);
+  }
+  __device__ __forceinline__ int holder(int64_t unit) const {
+    const int64_t big = more * (each + 1);
+    return (int)(unit < big ? div64(unit, each + 1) : more + div64(unit - big, each));
+  }
+};
+
 template <int D, bool F8, bool CAP>
-__global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttn p) {
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttn p) {
   using S = DecShape<D, F8>;
-  constexpr int LDO = D + 4;
-  __shared__ __align__(16) float sO[4 * kDecRows * LDO];
-  __shared__ float sM[4][kDecRows], sL[4][kDecRows];
+  constexpr int LDO = D + 4, NTH = 64 * kWaves;
+  __shared__ __align__(16) float sO[kWaves * kDecRows * LDO];
+  __shared__ float sM[kWaves][kDecRows], sL[kWaves][kDecRows];
+  // head dim 256: the queries, whose registers the loads in flight need
+  constexpr bool QL = D == 256;
+  __shared__ __align__(16) bf16_t sQ[QL ? S::NS * 64 * 8 : 8];
   __shared__ int sPid[kPageIds + 4];
-  __shared__ int64_t sScan[4];
+  __shared__ int64_t sScan[kWaves];
   __shared__ int64_t sBase;
   __shared__ int sSeq;
 
@@ -140,109 +186,146 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttn p) {
   const int wg = blockIdx.x, n_wg = gridDim.x;
   const int lg = p.b.lg_page, G = p.group;
 
-  // Units of sequence b: key/value heads x 16-row tiles x units of its keys
-  // (one for a sequence that sees nothing: its rows are still written).
-  auto seq_units = [&](int b, int& per, int& tiles) {
-    PagedSeq s;
-    s.load(p, b);
+  // A sequence's units: key/value heads x 16-row tiles x `per` units of its
+  // keys (one if it sees nothing: its rows are still written).
+  struct Units {
+    int per, tiles;
+    int64_t all;
+  };
+  auto units_of = [&](const PagedSeq& s) {
+    Units u;
     const int64_t rows = (int64_t)s.n * G;
-    tiles = rows <= p.most_rows ? (int)((rows + kDecRows - 1) / kDecRows) : 0;
+    u.tiles = rows <= p.most_rows ? (int)((rows + kDecRows - 1) / kDecRows) : 0;
     int lo, hi, x;
     s.keys(p, 0, lo, x);
     s.keys(p, s.n - 1, x, hi);
-    const int ub = S::KB * kUnitBlocks;
-    per = hi > lo ? (hi + ub - 1) / ub - lo / ub : 1;
-    return (int64_t)per * tiles * p.kv_heads;
+    u.per = hi > lo ? (hi + S::UB - 1) / S::UB - lo / S::UB : 1;
+    u.all = (int64_t)u.per * u.tiles * p.kv_heads;
+    return u;
   };
 
-  // this workgroup's piece [g0, g1) of all units, and the sequence of g0
-  int64_t g0, g1, total;
-  int wgs;
+  // this workgroup's piece [g0, g1) of all units, and the sequence of g0: up
+  // to 64 sequences by every wave for itself, a lane each; more by the
+  // workgroup, a run of sequences per thread
+  int64_t total = 0, base = 0, g0, g1;
+  int b = 0;
+  PagedSeq s;
+  const bool lanes = p.b.n_seqs <= 64;
+  int64_t at = 0, mine = 0;
+  const int each = lanes ? 1 : (p.b.n_seqs + NTH - 1) / NTH, first = (lanes ? lane : tid) * each;
+  for (int i = 0; i < each; ++i)
+    if (first + i < p.b.n_seqs) {
+      s.load(p, first + i);
+      mine += units_of(s).all;
+    }
   {
-    const int each = (p.b.n_seqs + 255) / 256, first = tid * each;
-    int64_t mine = 0;
-    int per, tiles;
-    for (int i = 0; i < each; ++i)
-      if (first + i < p.b.n_seqs) mine += seq_units(first + i, per, tiles);
     int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int64_t v = __shfl_up(incl, o, 64);
       if (lane >= o) incl += v;
     }
-    if (lane == 63) sScan[wave] = incl;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
+    at = incl - mine;
+    total = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(incl >> 32), 63) << 32) |
+                      (uint32_t)__builtin_amdgcn_readlane((int)incl, 63));
+    if (!lanes) {
+      if (lane == 63) sScan[wave] = incl;
+      __syncthreads();
+      total = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i < wave) before += sScan[i];
-      total += sScan[i];
-    }
-    wgs = total < n_wg ? (int)total : n_wg;
-    if (wg >= wgs) {
-      if (tid == 0) p.rec[wg * 8] = -1;
-      return;
-    }
-    g0 = total * wg / wgs;
-    g1 = total * (wg + 1) / wgs;
-    int64_t at = before + incl - mine;
-    if (g0 >= at && g0 < at + mine) {
-      int b = first;
-      for (;; ++b) {
-        const int64_t u = seq_units(b, per, tiles);
-        if (g0 < at + u) break;
-        at += u;
+      for (int i = 0; i < kWaves; ++i) {
+        if (i < wave) at += sScan[i];
+        total += sScan[i];
       }
-      sSeq = b;
+    }
+  }
+  const int wgs = total < n_wg ? (int)total : n_wg;
+  if (wg >= wgs) {
+    if (tid == 0) p.rec[wg * 8] = -1;
+    return;
+  }
+  const Pieces pieces(total, wgs);
+  g0 = pieces.start(wg);
+  g1 = pieces.start(wg + 1);
+  if (lanes) {
+    b = __builtin_ctzll(__ballot(g0 >= at && g0 < at + mine));
+    base = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), b) << 32) |
+                     (uint32_t)__builtin_amdgcn_readlane((int)at, b));
+    s.q0 = __builtin_amdgcn_readlane(s.q0, b);
+    s.n = __builtin_amdgcn_readlane(s.n, b);
+    s.raw = __builtin_amdgcn_readlane(s.raw, b);
+    s.len = __builtin_amdgcn_readlane(s.len, b);
+    s.pre = __builtin_amdgcn_readlane(s.pre, b);
+  } else {
+    if (g0 >= at && g0 < at + mine) {
+      int c = first;
+      for (;; ++c) {
+        s.load(p, c);
+        const int64_t n = units_of(s).all;
+        if (g0 < at + n) break;
+        at += n;
+      }
+      sSeq = c;
       sBase = at;
     }
     __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(sSeq);
+    base = sBase;
+    base = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(base >> 32)) << 32) |
+                     (uint32_t)__builtin_amdgcn_readfirstlane((int)base));
+    s.load(p, b);
   }
-
-  int b = sSeq;
-  int64_t base = sBase, at = g0;
-  bool crosses = false;
+  Units u = units_of(s);
+  bool crosses = false, again = false;
+  at = g0;
   while (at < g1) {
-    int per, tiles;
-    const int64_t units = seq_units(b, per, tiles);
-    if (at >= base + units) {
-      base += units;
-      ++b;
+    if (at >= base + u.all) {
+      base += u.all;
+      s.load(p, ++b);
+      u = units_of(s);
       continue;
     }
     // problem j of the sequence (key/value head fastest), its units [u0, u1)
-    const int j = (int)((at - base) / per);
-    const int h = j % p.kv_heads, rt = j / p.kv_heads;
+    const int per = u.per;
+    const int j = (int)div64(at - base, per);
+    const int rt = j / p.kv_heads, h = j - rt * p.kv_heads;
     const int64_t p0 = base + (int64_t)j * per, p1 = p0 + per;
     const int u0 = (int)(at - p0), u1 = (int)((p1 < g1 ? p1 : g1) - p0);
     const bool whole = p0 >= g0 && p1 <= g1;
 
-    PagedSeq s;
-    s.load(p, b);
     const int rows = s.n * G - rt * kDecRows < kDecRows ? s.n * G - rt * kDecRows : kDecRows;
     // this lane's row, its keys, and those of the first and last row
     const int r = rt * kDecRows + (m < rows ? m : rows - 1);
-    const int tok = r / G, head = h * G + r - tok * G;
+    const int tok = p.by_group.div(r), head = h * G + r - tok * G;
     int lo, hi, lo_min, lo_max, hi_min, hi_max, seq_lo, x;
     s.keys(p, tok, lo, hi);
-    s.keys(p, rt * kDecRows / G, lo_min, hi_min);
-    s.keys(p, (rt * kDecRows + rows - 1) / G, lo_max, hi_max);
+    s.keys(p, p.by_group.div(rt * kDecRows), lo_min, hi_min);
+    s.keys(p, p.by_group.div(rt * kDecRows + rows - 1), lo_max, hi_max);
     s.keys(p, 0, seq_lo, x);
-    constexpr int UB = S::KB * kUnitBlocks;
-    const int k_first = (seq_lo / UB + u0) * UB, k_last = (seq_lo / UB + u1) * UB;
+    const int k_first = (seq_lo / S::UB + u0) * S::UB, k_last = (seq_lo / S::UB + u1) * S::UB;
     // key blocks of this piece that some row sees
     const int kb0 = (k_first > lo_min ? k_first : lo_min) / S::KB;
     const int k_end = k_last < hi_max ? k_last : hi_max;
     const int kb1 = (k_end + S::KB - 1) / S::KB;
 
-    bf16x8 qf[S::NS];
+    // Q's fragment i: dims 32 i + 8 g ... of row m (e4m3: the order of the
+    // keys' loads, 16 dims of a pair of fragments per lane)
+    bf16x8 qf[QL ? 1 : S::NS];
     {
       const bf16_t* qr = p.q + (int64_t)(s.q0 + tok) * p.ldq + (int64_t)head * D;
+      auto dim = [&](int i) { return F8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g; };
+      if constexpr (QL) {
+        static_assert(!QL || S::NS == kWaves, "a fragment per wave");
+        st8(&sQ[(wave * 64 + lane) * 8], ld8(qr + dim(wave)));
+      } else {
 #pragma unroll
-      for (int i = 0; i < S::NS; ++i)
-        qf[i] = ld8(qr + (F8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g));
+        for (int i = 0; i < S::NS; ++i) qf[i] = ld8(qr + dim(i));
+      }
     }
+    auto q_frag = [&](int i) {
+      if constexpr (QL) return ld8(&sQ[(i * 64 + lane) * 8]);
+      else return qf[i];
+    };
     float sc = p.scale * (F8 && p.k_scale ? p.k_scale[h] : 1.f);
     // CAP: cap tanh(x / cap) = cap (1 - 2 / (exp(2 x / cap) + 1))
     sc *= CAP ? 2.f * kLog2e / p.softcap : kLog2e;
@@ -262,8 +345,9 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttn p) {
       const int c1 = c0 + CB < kb1 ? c0 + CB : kb1;
       const int pg0 = (int)(((int64_t)c0 * S::KB) >> lg);
       const int pg1 = (int)(((int64_t)c1 * S::KB - 1) >> lg);
-      __syncthreads();
-      for (int i = tid; i <= pg1 - pg0; i += 256) sPid[i] = paged_page(p.b, b, pg0 + i);
+      if (again) __syncthreads();  // the ids before these are read
+      again = true;
+      for (int i = tid; i <= pg1 - pg0; i += NTH) sPid[i] = paged_page(p.b, b, pg0 + i);
       __syncthreads();
 
       auto load_k = [&](int kb) {
@@ -296,15 +380,15 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttn p) {
 #pragma unroll
           for (int t = 0; t < S::NT; ++t) {
             if constexpr (F8) {
-              sa[t] = mfma16x16x32(e4m3x8_to_bf16(kr[t][i].w[0], kr[t][i].w[1]), qf[2 * i], sa[t]);
-              sa[t] = mfma16x16x32(e4m3x8_to_bf16(kr[t][i].w[2], kr[t][i].w[3]), qf[2 * i + 1], sa[t]);
+              sa[t] = mfma16x16x32(e4m3x8_to_bf16(kr[t][i].w[0], kr[t][i].w[1]), q_frag(2 * i), sa[t]);
+              sa[t] = mfma16x16x32(e4m3x8_to_bf16(kr[t][i].w[2], kr[t][i].w[3]), q_frag(2 * i + 1), sa[t]);
             } else {
-              sa[t] = mfma16x16x32(kr[t][i], qf[i], sa[t]);
+              sa[t] = mfma16x16x32(kr[t][i], q_frag(i), sa[t]);
             }
           }
         // (the next block's keys take the registers of this one's, not others)
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (decltype(more)::value) load_k(kb + 4);
+        if constexpr (decltype(more)::value) load_k(kb + kWaves);
         __builtin_amdgcn_sched_barrier(0);
 
         const int k0 = kb * S::KB, kg = k0 + S::GS * g;
@@ -373,19 +457,19 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttn p) {
           }
         }
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (decltype(more)::value) load_v(kb + 4);
+        if constexpr (decltype(more)::value) load_v(kb + kWaves);
         __builtin_amdgcn_sched_barrier(0);
       };
       int kb = c0 + wave;
-      if (kb < c1) {
+      if (kb < c1) {  // (all of it in one branch: exact waits for the loads)
         load_k(kb);
         load_v(kb);
-        for (; kb + 4 < c1; kb += 4) block(kb, BoolC<true>{});
+        for (; kb + kWaves < c1; kb += kWaves) block(kb, BoolC<true>{});
         block(kb, BoolC<false>{});
       }
     }
 
-    // the four waves' rows together: weights exp2(m_w - M)
+    // the waves' rows together: weights exp2(m_w - M)
     l_run = quad_sum(l_run);
     if (g == 0) {
       sM[wave][m] = m_run;
@@ -404,24 +488,24 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttn p) {
     __syncthreads();
     const int slot = at > g0 ? 1 : 0;
     float* part = p.part + ((int64_t)wg * 2 + slot) * S::PF;
-    for (int c = tid; c < rows * (D / 4); c += 256) {
+    for (int c = tid; c < rows * (D / 4); c += NTH) {
       const int i = c / (D / 4), d0 = (c % (D / 4)) * 4;
-      float top = sM[0][i];
+      float mw[kWaves], top = -INFINITY;
 #pragma unroll
-      for (int w = 1; w < 4; ++w) top = fmaxf(top, sM[w][i]);
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, mw[w] = sM[w][i]);
       f32x4_t a = f32x4_t{0.f, 0.f, 0.f, 0.f};
       float l = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if (sM[w][i] == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(sM[w][i] - top);
+      for (int w = 0; w < kWaves; ++w) {
+        // (a wave without keys holds zeros)
+        const float f = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[w] - top);
         const f32x4_t t = *(const f32x4_t*)&sO[(w * kDecRows + i) * LDO + d0];
         l += f * sL[w][i];
 #pragma unroll
         for (int e = 0; e < 4; ++e) a[e] += f * t[e];
       }
       if (whole) {
-        const int rr = rt * kDecRows + i, tk = rr / G;
+        const int rr = rt * kDecRows + i, tk = p.by_group.div(rr);
         const float inv = l > 0.f ? 1.f / l : 0.f;
         uint2 w2;
         w2.x = f2bf2(a[0] * inv, a[1] * inv);
@@ -442,7 +526,7 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttn p) {
       crosses = true;
       if (tid == 0) {
         int32_t* rec = p.rec + wg * 8;
-        rec[0] = (int)((p1 * wgs - 1) / total);  // the workgroup of its last unit
+        rec[0] = pieces.holder(p1 - 1);  // the workgroup of its last unit
         rec[1] = slot;
         rec[2] = s.q0;
         rec[3] = rt;
@@ -457,13 +541,13 @@ __global__ __launch_bounds__(256, 2) void paged_decode_kernel(PagedAttn p) {
 
 // Rows blockIdx.y, + gridDim.y, ... of the problem that crosses out of
 // workgroup blockIdx.x: its partials (slot rec[1] there, slot 0 in the
-// workgroups after it) are added in a fixed order, a quarter (256 / (D / 4)
-// groups) of them per group of threads, weighted by exp2(m_w - M).
-template <int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn p) {
-  constexpr int V = D / 4, NG = 256 / V;
+// workgroups after it) weighted by exp2(m_w - M), and added by NT / (D / 4)
+// groups of threads, then over the groups, in a fixed order.
+template <int D, int NT>
+__global__ __launch_bounds__(NT) void paged_merge_kernel(PagedAttn p) {
+  constexpr int V = D / 4, NG = NT / V;
   constexpr int64_t PF = kDecRows * (D + 2);
-  __shared__ float sT[4];
+  __shared__ float sT[NT / 64];
   __shared__ __align__(16) float sA[NG][D];
   __shared__ float sW[NG];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -478,16 +562,17 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn p) {
   };
   for (int i = blockIdx.y; i < rows; i += gridDim.y) {
     float top = -INFINITY;
-    for (int w = tid; w < n; w += 256) top = fmaxf(top, partial(w)[kDecRows * D + i]);
+    for (int w = tid; w < n; w += NT) top = fmaxf(top, partial(w)[kDecRows * D + i]);
     top = wave_max(top);
     __syncthreads();  // the previous row's sums are read
     if (lane == 0) sT[wave] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(sT[0], sT[1]), fmaxf(sT[2], sT[3]));
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) top = fmaxf(top, sT[w]);
     const int v = tid % V, gr = tid / V;
     f32x4_t a = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int w = gr; w < n; w += NG) {
       const float* pt = partial(w);
       const float mw = pt[kDecRows * D + i];
@@ -501,17 +586,17 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn p) {
     if (v == 0) sW[gr] = l;
     __syncthreads();
     if (tid < V) {
+      const int groups = n < NG ? n : NG;
       float den = 0.f;
       f32x4_t t = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < NG; ++u) {
+      for (int u = 0; u < groups; ++u) {
         den += sW[u];
         const f32x4_t x = *(const f32x4_t*)&sA[u][4 * tid];
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] += x[e];
       }
       const float inv = den > 0.f ? 1.f / den : 0.f;
-      const int rr = rt * kDecRows + i, tk = rr / p.group;
+      const int rr = rt * kDecRows + i, tk = p.by_group.div(rr);
       uint2 w2;
       w2.x = f2bf2(t[0] * inv, t[1] * inv);
       w2.y = f2bf2(t[2] * inv, t[3] * inv);
@@ -727,8 +812,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   const int all = s.n * G;
   const int r_tile = rt * S::BM, rows = all - r_tile < S::BM ? all - r_tile : S::BM;
   int lo_min, lo_tile, hi_tile, hi_max;
-  s.keys(p, r_tile / G, lo_min, hi_tile);
-  s.keys(p, (r_tile + rows - 1) / G, lo_tile, hi_max);
+  s.keys(p, p.by_group.div(r_tile), lo_min, hi_tile);
+  s.keys(p, p.by_group.div(r_tile + rows - 1), lo_tile, hi_max);
   // tiles of this key range
   int t0 = lo_min / kProTile, t1 = (hi_max + kProTile - 1) / kProTile;
   if (t1 < t0) t1 = t0;
@@ -753,7 +838,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   for (int n = 0; n < NR; ++n) {
     const int i = 32 * NR * w + 32 * n + qi;
     const int r = r_tile + (i < rows ? i : rows - 1);
-    tok[n] = r / G;
+    tok[n] = p.by_group.div(r);
     head[n] = h * G + r - tok[n] * G;
     s.keys(p, tok[n], lo[n], hi[n]);
     const bf16_t* qr = p.q + (int64_t)(s.q0 + tok[n]) * p.ldq + (int64_t)head[n] * D;
@@ -771,8 +856,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     int x;
     const int last = r_wave + 32 * NR - 1 < r_tile + rows - 1 ? r_wave + 32 * NR - 1
                                                               : r_tile + rows - 1;
-    s.keys(p, r_wave / G, x, hi_min);
-    s.keys(p, last / G, lo_max, x);
+    s.keys(p, p.by_group.div(r_wave), x, hi_min);
+    s.keys(p, p.by_group.div(last), lo_max, x);
   }
 
   // O^T, the scores of a tile's halves (sa[half]) and their probabilities
@@ -1169,47 +1254,44 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   }
 }
 
-// The key ranges of a problem together, in their order: rows 16 blockIdx.y
-// ... of problem blockIdx.x.
+// The key ranges of a problem together, in their order: one thread per four
+// dims of a row, rows 256 / (D / 4) blockIdx.y ... of problem blockIdx.x.
 template <int D>
 __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(PagedAttn p) {
   using S = ProShape<D, false>;
   const int prob = blockIdx.x, rows = p.prec[prob * 4];
-  if ((int)blockIdx.y * 16 >= rows) return;
+  const int i = blockIdx.y * (1024 / D) + threadIdx.x / (D / 4), d0 = threadIdx.x % (D / 4) * 4;
+  if (i >= rows) return;
   const int q0 = p.prec[prob * 4 + 1], r_tile = p.prec[prob * 4 + 2], h = p.prec[prob * 4 + 3];
   const float* part = p.ppart + (int64_t)prob * p.splits * S::PF;
-  for (int c = threadIdx.x; c < 16 * (D / 4); c += 256) {
-    const int i = blockIdx.y * 16 + c / (D / 4), d0 = (c % (D / 4)) * 4;
-    if (i >= rows) break;
-    float top = -INFINITY;
-    for (int k = 0; k < p.splits; ++k) top = fmaxf(top, part[(int64_t)k * S::PF + S::BM * D + i]);
-    f32x4_t a = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < p.splits; ++k) {
-      const float* x = part + (int64_t)k * S::PF;
-      const float m = x[S::BM * D + i];
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-      const f32x4_t t = *(const f32x4_t*)(x + i * D + d0);
-      l += f * x[S::BM * D + S::BM + i];
+  float top = -INFINITY;
+#pragma unroll 8
+  for (int k = 0; k < p.splits; ++k) top = fmaxf(top, part[(int64_t)k * S::PF + S::BM * D + i]);
+  f32x4_t a = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < p.splits; ++k) {
+    const float* x = part + (int64_t)k * S::PF;
+    const float m = x[S::BM * D + i];
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    const f32x4_t t = *(const f32x4_t*)(x + i * D + d0);
+    l += f * x[S::BM * D + S::BM + i];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) a[e] += f * t[e];
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int r = r_tile + i, tk = r / p.group;
-    uint2 v;
-    v.x = f2bf2(a[0] * inv, a[1] * inv);
-    v.y = f2bf2(a[2] * inv, a[3] * inv);
-    *(uint2*)(p.o + (int64_t)(q0 + tk) * p.ldo + (int64_t)(h * p.group + r - tk * p.group) * D + d0) = v;
+    for (int e = 0; e < 4; ++e) a[e] += f * t[e];
   }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int r = r_tile + i, tk = p.by_group.div(r);
+  uint2 v;
+  v.x = f2bf2(a[0] * inv, a[1] * inv);
+  v.y = f2bf2(a[2] * inv, a[3] * inv);
+  *(uint2*)(p.o + (int64_t)(q0 + tk) * p.ldo + (int64_t)(h * p.group + r - tk * p.group) * D + d0) = v;
 }
 
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-// Workgroups of the decode kernel: as many as run at once (two per CU by
-// registers).
-static int decode_wgs() { return 2 * device_cus(); }
+// Workgroups of the decode kernel: one per CU.
+static int decode_wgs() { return device_cus(); }
 
 // Which kernels a call launches, their grids and their parts of the
 // workspace.  The host knows the number of rows and sequences and, as a hint,
@@ -1259,18 +1341,25 @@ static void launch_many(const PagedAttn& p, bool f8, bool cap, hipStream_t s) {
   else hipLaunchKernelGGL((paged_prompt_kernel<D, false, false>), grid, block, 0, s, p);
   if (p.splits > 1)
     hipLaunchKernelGGL((paged_prompt_merge_kernel<D>),
-                       dim3((unsigned)p.problems, ProShape<D, false>::BM / 16), block, 0, s, p);
+                       dim3((unsigned)p.problems, ProShape<D, false>::BM * D / 1024), block, 0, s, p);
 }
 
 template <int D>
 static void launch_few(const PagedAttn& p, bool f8, bool cap, int n_wg, unsigned ry,
                        hipStream_t s) {
-  const dim3 grid((unsigned)n_wg), block(256);
+  const dim3 grid((unsigned)n_wg), block(64 * kWaves);
   if (f8 && cap) hipLaunchKernelGGL((paged_decode_kernel<D, true, true>), grid, block, 0, s, p);
   else if (f8) hipLaunchKernelGGL((paged_decode_kernel<D, true, false>), grid, block, 0, s, p);
   else if (cap) hipLaunchKernelGGL((paged_decode_kernel<D, false, true>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((paged_decode_kernel<D, false, false>), grid, block, 0, s, p);
-  hipLaunchKernelGGL((paged_merge_kernel<D>), dim3((unsigned)n_wg, ry), block, 0, s, p);
+  // Few problems of one sequence each: long lines of partials, more threads
+  // for each (256 partials of 8 x 256: 8.2 us with 1024 threads, 29 with 256;
+  // two partials of 4 x 128, 512 times: 9.1 and 4.7).
+  const dim3 merge((unsigned)n_wg, ry);
+  if ((int64_t)p.b.n_seqs * p.kv_heads * 8 < n_wg)
+    hipLaunchKernelGGL((paged_merge_kernel<D, 1024>), merge, dim3(1024), 0, s, p);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<D, 256>), merge, dim3(256), 0, s, p);
 }
 
 static int check_paged_attention(const fvx_paged_attn_desc* d) {
@@ -1363,6 +1452,7 @@ extern "C" int fvx_paged_attention(const fvx_paged_attn_desc* d, void* stream) {
   p.prefix_len = d->prefix_len;
   p.kv_heads = (int)d->kv_heads;
   p.group = (int)(d->q_heads / d->kv_heads);
+  p.by_group = FastDiv::of((uint32_t)p.group);
   p.window = (int)d->window;
   p.scale = d->scale;
   p.softcap = d->softcap;
