@@ -51,12 +51,13 @@ struct PagedAttn {
   const float* v_scale;
   const int32_t* prefix_len;
   int32_t kv_heads, group, window;
-  FastDiv by_group;
+  FastDiv by_group, by_kv;
   float scale, softcap;
   // few rows: sequences of at most most_rows query rows per key/value head
   int32_t most_rows;
+  int32_t by_problem;  // records by problem, not by workgroup
   int32_t extra;  // units that a problem counts beside its key blocks
-  int32_t* rec;  // [n_wg][8] problems that cross workgroups
+  int32_t* rec;  // [8 each] problems that cross workgroups
   float* part;   // [n_wg][2][16 rows x (D + 2)] partials
   // many rows: the others; problems and key ranges of the launch
   int32_t problems, splits;
@@ -89,21 +90,15 @@ struct PagedSeq {
   int q0, n, raw, len, pre;
   __device__ __forceinline__ void load(const PagedAttn& p, int b) {
     paged_rows(p.b, b, q0, n);
-    raw = p.b.kv_len[b];
+    raw = max(p.b.kv_len[b], 0);
     pre = p.prefix_len ? p.prefix_len[b] : 0;
-    const int64_t most = (int64_t)p.b.max_pages << p.b.lg_page;
-    len = raw < 0 ? 0 : (raw < most ? raw : (int)most);
+    len = min(raw, p.b.max_pages << p.b.lg_page);
   }
   __device__ __forceinline__ void keys(const PagedAttn& p, int i, int& lo, int& hi) const {
-    const int64_t t = (int64_t)raw - n + i;
-    if (t < 0) {
-      lo = hi = 0;
-      return;
-    }
-    const int64_t h = t + 1 > pre ? t + 1 : pre;
-    hi = h < len ? (int)h : len;
-    const int64_t l = p.window > 0 ? t - p.window + 1 : 0;
-    lo = l < 0 ? 0 : (l < hi ? (int)l : hi);
+    const int t = raw - n + i;  // below raw
+    hi = t < 0 ? 0 : min(max(t + 1, pre), len);
+    lo = clampi(p.window > 0 ? t - p.window + 1 : 0, 0, hi);
+    lo = t < 0 ? 0 : lo;
   }
 };
 
@@ -242,7 +237,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttn 
   }
   const int wgs = total < n_wg ? (int)total : n_wg;
   if (wg >= wgs) {
-    if (tid == 0) p.rec[wg * 8] = -1;
+    if (tid == 0 && !p.by_problem) p.rec[wg * 8] = -1;
     return;
   }
   const Pieces pieces(total, wgs);
@@ -277,7 +272,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttn 
     s.load(p, b);
   }
   Units u = units_of(s);
-  bool crosses = false, again = false;
+  bool starts = false, again = false;  // a problem starts here
   at = g0;
   while (at < g1) {
     if (at >= base + u.all) {
@@ -288,11 +283,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttn 
     }
     // problem j of the sequence (key/value head fastest), its units [u0, u1)
     const int per = u.per;
-    const int j = (int)div64(at - base, per);
-    const int rt = j / p.kv_heads, h = j - rt * p.kv_heads;
+    const int j = at - base < per ? 0 : (int)div64(at - base, per);
+    const int rt = p.by_kv.div(j), h = j - rt * p.kv_heads;
     const int64_t p0 = base + (int64_t)j * per, p1 = p0 + per;
     const int u0 = (int)(at - p0), u1 = (int)((p1 < g1 ? p1 : g1) - p0);
     const bool whole = p0 >= g0 && p1 <= g1;
+    starts = starts || p0 >= g0;
 
     const int rows = s.n * G - rt * kDecRows < kDecRows ? s.n * G - rt * kDecRows : kDecRows;
     // this lane's row, its keys, and those of the first and last row
@@ -374,7 +370,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttn 
             p.v + (((((int64_t)(vpid < 0 ? 0 : vpid) * p.kv_heads + h) * D + m) << lg) +
                    (key & ((1 << lg) - 1))) * S::ES;
 #pragma unroll
-        for (int d = 0; d < S::ND; ++d) vr[d] = *(const bf16x8*)(a + ((int64_t)(d * 16 * S::ES) << lg));
+        for (int d = 0; d < S::ND; ++d) {
+          vr[d] = *(const bf16x8*)a;
+          a += (uint32_t)(16 * S::ES) << lg;
+        }
       };
       auto block = [&](int kb, auto more) {
         f32x4_t sa[S::NT];
@@ -527,26 +526,28 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(PagedAttn 
     __syncthreads();  // the rows in LDS are read
     // a problem that starts here and ends in a later workgroup: what the
     // merge has to know
-    if (p1 > g1 && p0 >= g0) {
-      crosses = true;
-      if (tid == 0) {
-        int32_t* rec = p.rec + wg * 8;
-        rec[0] = pieces.holder(p1 - 1);  // the workgroup of its last unit
+    if (p0 >= g0 && tid == 0) {
+      int32_t* rec = p.rec + (p.by_problem ? (b * u.tiles + rt) * p.kv_heads + h : wg) * 8;
+      if (p1 > g1) {
+        rec[0] = pieces.holder(p1 - 1) - wg + 1;  // workgroups
         rec[1] = slot;
         rec[2] = s.q0;
         rec[3] = rt;
         rec[4] = h;
         rec[5] = rows;
+        rec[6] = wg;
+      } else {
+        rec[0] = -1;
       }
     }
     at = p0 + u1;
   }
-  if (!crosses && tid == 0) p.rec[wg * 8] = -1;
+  if (!p.by_problem && !starts && tid == 0) p.rec[wg * 8] = -1;
 }
 
-// Rows blockIdx.y, + gridDim.y, ... of the problem that crosses out of
-// workgroup blockIdx.x: its partials (slot rec[1] there, slot 0 in the
-// workgroups after it) weighted by exp2(m_w - M), and added by NT / (D / 4)
+// Rows blockIdx.y, + gridDim.y, ... of the problem of record blockIdx.x, if it
+// crosses workgroups: its partials (slot rec[1] of workgroup rec[6], slot 0 of
+// the ones after it) weighted by exp2(m_w - M), and added by NT / (D / 4)
 // groups of threads, then over the groups, in a fixed order.
 template <int D, int NT>
 __global__ __launch_bounds__(NT) void paged_merge_kernel(PagedAttn p) {
@@ -556,12 +557,10 @@ __global__ __launch_bounds__(NT) void paged_merge_kernel(PagedAttn p) {
   __shared__ __align__(16) float sA[NG][D];
   __shared__ float sW[NG];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int first = blockIdx.x;
-  const int32_t* rec = p.rec + first * 8;
-  const int last = rec[0];
-  if (last < 0) return;
-  const int slot = rec[1], q0 = rec[2], rt = rec[3], h = rec[4], rows = rec[5];
-  const int n = last - first + 1;
+  const int32_t* rec = p.rec + (int64_t)blockIdx.x * 8;
+  const int n = rec[0];
+  if (n < 0) return;
+  const int slot = rec[1], q0 = rec[2], rt = rec[3], h = rec[4], rows = rec[5], first = rec[6];
   auto partial = [&](int i) {
     return p.part + ((int64_t)(first + i) * 2 + (i == 0 ? slot : 0)) * PF;
   };
@@ -773,7 +772,7 @@ __device__ bool find_tile(const PagedAttn& p, int item, int64_t* scan, int* foun
     if (i < wave) before += scan[i];
     total += scan[i];
   }
-  const int want = item / p.kv_heads;
+  const int want = p.by_kv.div(item);
   h = item - want * p.kv_heads;
   if (want >= total) return false;
   int64_t at = before + incl - mine;
@@ -1357,10 +1356,11 @@ static void launch_few(const PagedAttn& p, bool f8, bool cap, int n_wg, unsigned
   else if (f8) hipLaunchKernelGGL((paged_decode_kernel<D, true, false>), grid, block, 0, s, p);
   else if (cap) hipLaunchKernelGGL((paged_decode_kernel<D, false, true>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((paged_decode_kernel<D, false, false>), grid, block, 0, s, p);
-  // Few problems of one sequence each: long lines of partials, more threads
-  // for each (256 partials of 8 x 256: 8.2 us with 1024 threads, 29 with 256;
-  // two partials of 4 x 128, 512 times: 9.1 and 4.7).
-  const dim3 merge((unsigned)n_wg, ry);
+  // Few problems: long lines of partials, more threads for each (256 partials
+  // of 8 x 256: 8.2 us with 1024 threads, 29 with 256; two partials of 4 x
+  // 128, 512 times: 9.1 and 4.7).
+  const int64_t tiles = (p.group + kDecRows - 1) / kDecRows;
+  const dim3 merge(p.by_problem ? (unsigned)(p.b.n_seqs * tiles * p.kv_heads) : (unsigned)n_wg, ry);
   if ((int64_t)p.b.n_seqs * p.kv_heads * 8 < n_wg)
     hipLaunchKernelGGL((paged_merge_kernel<D, 1024>), merge, dim3(1024), 0, s, p);
   else
@@ -1458,6 +1458,7 @@ extern "C" int fvx_paged_attention(const fvx_paged_attn_desc* d, void* stream) {
   p.kv_heads = (int)d->kv_heads;
   p.group = (int)(d->q_heads / d->kv_heads);
   p.by_group = FastDiv::of((uint32_t)p.group);
+  p.by_kv = FastDiv::of((uint32_t)p.kv_heads);
   p.window = (int)d->window;
   p.scale = d->scale;
   p.softcap = d->softcap;
@@ -1469,6 +1470,9 @@ extern "C" int fvx_paged_attention(const fvx_paged_attn_desc* d, void* stream) {
   p.extra = d->n_seqs * d->kv_heads >= plan.n_wg
                 ? (int)((128 << 10) / (2 * d->head_dim * 64)) : 0;
   p.most_rows = plan.most_rows;
+  // one row per sequence: the problems are known; fewer than workgroups, each
+  // has its record
+  p.by_problem = !d->q_start && d->n_seqs * ((p.group + kDecRows - 1) / kDecRows) * d->kv_heads < plan.n_wg;
   p.rec = (int32_t*)(ws + plan.rec);
   p.part = (float*)(ws + plan.part);
   p.problems = (int)plan.problems;

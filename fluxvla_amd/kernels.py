@@ -7,6 +7,7 @@ unless the caller omits an ``out=`` tensor, so calls with preallocated
 outputs are safe inside HIP graph capture.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -908,6 +909,8 @@ def _paged_batch(cache, page_table, kv_len, q_start, rows, ref):
 def _head_rows(t, name, heads, dim):
     """(rows, row stride) of [rows, heads, dim] or [rows, heads * dim] with
     the heads side by side."""
+    if t.is_contiguous() and tuple(t.shape[1:]) in ((heads, dim), (heads * dim,)):
+        return t.shape[0], heads * dim
     if t.dim() == 3 and tuple(t.shape[1:]) == (heads, dim):
         side = (heads == 1 or t.stride(1) == dim) and t.stride(2) == 1
     elif t.dim() == 2 and t.shape[1] == heads * dim:
@@ -927,8 +930,10 @@ def _head_rows(t, name, heads, dim):
 
 def _call_on(name, desc, device):
     """Entry point ``name`` on ``device`` and its current stream."""
-    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-    if device.index == torch.cuda.current_device():
+    index = device.index
+    # (torch.cuda.current_stream(device).cuda_stream, without the object)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch.cuda.current_device():
         _lib.call(name, ctypes.byref(desc), stream)
     else:
         with torch.cuda.device(device):
@@ -994,7 +999,7 @@ def paged_attention(q, cache, page_table, kv_len, out=None, q_start=None,
     ``softcap`` c > 0: scores c * tanh(s / c).  A token that sees nothing
     gives zeros; rows behind the last sequence are left as they were.
     ``max_q``: the most new tokens of one sequence when known (a hint).
-    workspace: uint8 of paged_attention_workspace_bytes, taken from the
+    ``workspace``: uint8 [paged_attention_workspace_bytes], taken from the
     allocator unless given; calls on different streams need their own."""
     _check(q, 'q', contiguous=False)
     if q.dim() != 3:
@@ -1020,8 +1025,8 @@ def paged_attention(q, cache, page_table, kv_len, out=None, q_start=None,
         pages, max_q, cache.n_pages, cache.page_size, heads, kv, d, window,
         d ** -0.5 if scale is None else scale, softcap, cache.e4m3)
     if workspace is None:
-        workspace = torch.empty(_paged_ws_bytes(desc, q.device), dtype=torch.uint8,
-                                device=q.device)
+        size = _paged_ws_bytes(q.device.index, rows, n_seqs, starts is not None, max_q, heads, kv, d)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
     else:
         _check(workspace, 'workspace', dtype=torch.uint8)
         _same_device(q, workspace=workspace)
@@ -1030,13 +1035,22 @@ def paged_attention(q, cache, page_table, kv_len, out=None, q_start=None,
     return out
 
 
-def _paged_ws_bytes(desc, device):
-    fn = _lib.load().fvx_paged_attention_workspace_bytes
-    if device.index == torch.cuda.current_device():
-        n = fn(ctypes.byref(desc))
-    else:
-        with torch.cuda.device(device):
-            n = fn(ctypes.byref(desc))
+def paged_attention_workspace_bytes(q, cache, n_seqs, q_start=True, max_q=0):
+    """Workspace bytes of paged_attention for queries like ``q`` of
+    ``n_seqs`` sequences (``q_start``: whether it is given)."""
+    return _paged_ws_bytes(q.device.index, q.shape[0], n_seqs, bool(q_start),
+                           max_q if q_start else 1, q.shape[1], cache.kv_heads, cache.head_dim)
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_ws_bytes(index, rows, n_seqs, starts, max_q, heads, kv, d):
+    """fvx_paged_attention_workspace_bytes on device ``index`` (the sizes
+    that do not enter it are any)."""
+    desc = PagedAttnDesc(n_rows=rows, n_seqs=n_seqs, max_q=max_q, q_heads=heads, kv_heads=kv,
+                         head_dim=d, n_pages=1, page_size=16, q_start=16 if starts else None,
+                         scale=1.0)
+    with torch.cuda.device(index):
+        n = _lib.load().fvx_paged_attention_workspace_bytes(ctypes.byref(desc))
     if n < 0:
         raise ValueError(f'fvx_paged_attention: '
                          f'{_lib.load().fvx_last_error().decode(errors="replace")} (status {n})')
