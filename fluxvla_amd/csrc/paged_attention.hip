@@ -745,38 +745,49 @@ __device__ __forceinline__ int swz(int row, int c) {
 // more than most_rows rows, key/value head fastest, a sequence's last tile
 // (which sees most keys) first.  Returns false past the last one.
 template <int BM>
-__device__ bool find_tile(const PagedAttn& p, int item, int64_t* scan, int* found, int& b, int& t,
+__device__ bool find_tile(const PagedAttn& p, int item, int* scan, int* found, int& b, int& t,
                           int& h) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int each = (p.b.n_seqs + 255) / 256, first = tid * each;
+  // up to 64 sequences: every wave by itself, a lane each; more: a run of
+  // sequences per thread
+  const bool lanes = p.b.n_seqs <= 64;
+  const int each = lanes ? 1 : (p.b.n_seqs + 255) / 256, first = (lanes ? lane : tid) * each;
   auto tiles = [&](int s) {
     int q0, n;
     paged_rows(p.b, s, q0, n);
     const int64_t rows = (int64_t)n * p.group;
     return rows > p.most_rows ? (int)((rows + BM - 1) / BM) : 0;
   };
-  int64_t mine = 0;
+  int mine = 0;  // (problems are fewer than 2^31)
   for (int i = 0; i < each; ++i)
     if (first + i < p.b.n_seqs) mine += tiles(first + i);
-  int64_t incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t v = __shfl_up(incl, o, 64);
+    const int v = __shfl_up(incl, o, 64);
     if (lane >= o) incl += v;
   }
-  if (lane == 63) scan[wave] = incl;
-  __syncthreads();
-  int64_t before = 0, total = 0;
+  int at = incl - mine, total = __builtin_amdgcn_readlane(incl, 63);
+  if (!lanes) {
+    if (lane == 63) scan[wave] = incl;
+    __syncthreads();
+    total = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i < wave) before += scan[i];
-    total += scan[i];
+    for (int i = 0; i < 4; ++i) {
+      if (i < wave) at += scan[i];
+      total += scan[i];
+    }
   }
   const int want = p.by_kv.div(item);
   h = item - want * p.kv_heads;
   if (want >= total) return false;
-  int64_t at = before + incl - mine;
-  if (want >= at && want < at + mine) {
+  const bool here = want >= at && want < at + mine;
+  if (lanes) {
+    b = __builtin_ctzll(__ballot(here));
+    t = __builtin_amdgcn_readlane(mine - 1 - (want - at), b);
+    return true;
+  }
+  if (here) {
     int s = first, n;
     for (;; ++s) {
       n = tiles(s);
@@ -784,7 +795,7 @@ __device__ bool find_tile(const PagedAttn& p, int item, int64_t* scan, int* foun
       at += n;
     }
     found[0] = s;
-    found[1] = n - 1 - (int)(want - at);
+    found[1] = n - 1 - (want - at);
   }
   __syncthreads();
   b = __builtin_amdgcn_readfirstlane(found[0]);
@@ -798,8 +809,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   constexpr int NR = S::NR;
   __shared__ __align__(16) unsigned char smem[4 * S::TB];
   __shared__ int sPid[kProPages];
-  __shared__ int64_t sScan[4];
-  __shared__ int sFound[2], sMissing;
+  __shared__ int sScan[4], sFound[2], sMissing;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1258,28 +1268,53 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   }
 }
 
-// The key ranges of a problem together, in their order: one thread per four
-// dims of a row, rows 256 / (D / 4) blockIdx.y ... of problem blockIdx.x.
+// The key ranges of a problem together: rows blockIdx.y * 256 / D ... of
+// problem blockIdx.x, four dims per thread, a quarter of the ranges for each
+// of four groups of threads, which are then added in a fixed order.
 template <int D>
 __global__ __launch_bounds__(256) void paged_prompt_merge_kernel(PagedAttn p) {
   using S = ProShape<D, false>;
+  constexpr int V = D / 4, NR = 64 / V;  // threads of a row, rows per group
+  __shared__ __align__(16) float sA[4][NR][D];
+  __shared__ float sT[4][NR], sW[4][NR];
   const int prob = blockIdx.x, rows = p.prec[prob * 4];
-  const int i = blockIdx.y * (1024 / D) + threadIdx.x / (D / 4), d0 = threadIdx.x % (D / 4) * 4;
-  if (i >= rows) return;
+  const int gr = threadIdx.x / 64, ir = threadIdx.x % 64 / V, d0 = threadIdx.x % V * 4;
+  if ((int)blockIdx.y * NR >= rows) return;
+  const int i = blockIdx.y * NR + ir;
   const int q0 = p.prec[prob * 4 + 1], r_tile = p.prec[prob * 4 + 2], h = p.prec[prob * 4 + 3];
   const float* part = p.ppart + (int64_t)prob * p.splits * S::PF;
-  float top = -INFINITY;
-#pragma unroll 8
-  for (int k = 0; k < p.splits; ++k) top = fmaxf(top, part[(int64_t)k * S::PF + S::BM * D + i]);
+  float top = -INFINITY, l = 0.f;
   f32x4_t a = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-#pragma unroll 8
-  for (int k = 0; k < p.splits; ++k) {
-    const float* x = part + (int64_t)k * S::PF;
-    const float m = x[S::BM * D + i];
-    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-    const f32x4_t t = *(const f32x4_t*)(x + i * D + d0);
-    l += f * x[S::BM * D + S::BM + i];
+  if (i < rows) {
+#pragma unroll 4
+    for (int k = gr; k < p.splits; k += 4) {
+      const float* x = part + (int64_t)k * S::PF;
+      const float m = x[S::BM * D + i], w = x[S::BM * D + S::BM + i];
+      const f32x4_t t = *(const f32x4_t*)(x + i * D + d0);
+      const float nt = fmaxf(top, m);
+      const float fo = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - nt);
+      const float fn = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nt);
+      top = nt;
+      l = l * fo + fn * w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] = a[e] * fo + fn * t[e];
+    }
+  }
+  *(f32x4_t*)&sA[gr][ir][d0] = a;
+  if (d0 == 0) {
+    sT[gr][ir] = top;
+    sW[gr][ir] = l;
+  }
+  __syncthreads();
+  if (gr || i >= rows) return;
+  top = fmaxf(fmaxf(sT[0][ir], sT[1][ir]), fmaxf(sT[2][ir], sT[3][ir]));
+  l = 0.f;
+  a = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float f = sT[u][ir] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sT[u][ir] - top);
+    const f32x4_t t = *(const f32x4_t*)&sA[u][ir][d0];
+    l += f * sW[u][ir];
 #pragma unroll
     for (int e = 0; e < 4; ++e) a[e] += f * t[e];
   }
@@ -1325,8 +1360,15 @@ static PagedPlan paged_plan(const fvx_paged_attn_desc* d) {
   if (a.many) {
     const int64_t bm = 128;
     a.problems = (d->n_rows * G / bm + (d->n_seqs < d->n_rows ? d->n_seqs : d->n_rows)) * d->kv_heads;
-    // one workgroup per CU: with fewer problems their keys are split
-    const int64_t s = device_cus() / a.problems;
+    // With fewer problems than workgroups that run at once their keys are
+    // split, no finer than tiles of 64 keys and into 64 ranges at most, whose
+    // partials cost as much as they save (one sequence of 4000 keys, 40 rows
+    // of 256 dims: 62 us in 128 ranges).
+    const int64_t at_once = device_cus() * (d->head_dim == 256 ? 1 : 2);
+    const int64_t tiles = (d->max_pages * d->page_size + 63) / 64;
+    int64_t s = at_once / a.problems;
+    s = s < 64 ? s : 64;
+    s = s < tiles ? s : tiles;
     a.splits = s < 1 ? 1 : (int)s;
     if (a.splits > 1) {
       a.ppart = a.prec + (a.problems * 16 + 15) / 16 * 16;
@@ -1345,7 +1387,7 @@ static void launch_many(const PagedAttn& p, bool f8, bool cap, hipStream_t s) {
   else hipLaunchKernelGGL((paged_prompt_kernel<D, false, false>), grid, block, 0, s, p);
   if (p.splits > 1)
     hipLaunchKernelGGL((paged_prompt_merge_kernel<D>),
-                       dim3((unsigned)p.problems, ProShape<D, false>::BM * D / 1024), block, 0, s, p);
+                       dim3((unsigned)p.problems, ProShape<D, false>::BM * D / 256), block, 0, s, p);
 }
 
 template <int D>

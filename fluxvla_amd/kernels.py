@@ -1025,7 +1025,8 @@ def paged_attention(q, cache, page_table, kv_len, out=None, q_start=None,
         pages, max_q, cache.n_pages, cache.page_size, heads, kv, d, window,
         d ** -0.5 if scale is None else scale, softcap, cache.e4m3)
     if workspace is None:
-        size = _paged_ws_bytes(q.device.index, rows, n_seqs, starts is not None, max_q, heads, kv, d)
+        size = _paged_ws_bytes(q.device.index, rows, n_seqs, starts is not None, max_q, heads, kv, d,
+                               pages, cache.page_size)
         workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
     else:
         _check(workspace, 'workspace', dtype=torch.uint8)
@@ -1035,19 +1036,21 @@ def paged_attention(q, cache, page_table, kv_len, out=None, q_start=None,
     return out
 
 
-def paged_attention_workspace_bytes(q, cache, n_seqs, q_start=True, max_q=0):
-    """Workspace bytes of paged_attention for queries like ``q`` of
-    ``n_seqs`` sequences (``q_start``: whether it is given)."""
-    return _paged_ws_bytes(q.device.index, q.shape[0], n_seqs, bool(q_start),
-                           max_q if q_start else 1, q.shape[1], cache.kv_heads, cache.head_dim)
+def paged_attention_workspace_bytes(q, cache, page_table, q_start=None, max_q=0):
+    """Workspace bytes of paged_attention with these arguments (their
+    shapes; whether q_start is given)."""
+    return _paged_ws_bytes(q.device.index, q.shape[0], page_table.shape[0], q_start is not None,
+                           max_q if q_start is not None else 1, q.shape[1], cache.kv_heads,
+                           cache.head_dim, page_table.shape[1], cache.page_size)
 
 
 @functools.lru_cache(maxsize=4096)
-def _paged_ws_bytes(index, rows, n_seqs, starts, max_q, heads, kv, d):
+def _paged_ws_bytes(index, rows, n_seqs, starts, max_q, heads, kv, d, pages, page_size):
     """fvx_paged_attention_workspace_bytes on device ``index`` (the sizes
     that do not enter it are any)."""
     desc = PagedAttnDesc(n_rows=rows, n_seqs=n_seqs, max_q=max_q, q_heads=heads, kv_heads=kv,
-                         head_dim=d, n_pages=1, page_size=16, q_start=16 if starts else None,
+                         head_dim=d, n_pages=1, max_pages=pages, page_size=page_size,
+                         q_start=16 if starts else None,
                          scale=1.0)
     with torch.cuda.device(index):
         n = _lib.load().fvx_paged_attention_workspace_bytes(ctypes.byref(desc))
