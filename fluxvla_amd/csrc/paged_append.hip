@@ -2,9 +2,10 @@
 // positions, keys and values written into their pages.
 //
 // Bound by bytes: each Q|K|V value is read once and written once.  One
-// workgroup takes RB consecutive rows of one head.  Its Q|K|V loads do not
-// depend on where the rows go and are issued first; meanwhile one wave finds
-// the rows' sequences and pages.  Rotations are two products and a sum per
+// workgroup takes RB consecutive rows of HB query and key heads, or of one
+// value head.  Its first Q|K|V loads do not depend on where the rows go and
+// are issued first; meanwhile one wave finds the rows' sequences and pages.
+// The rows' rotations are read once for all its heads.  Rotations are two products and a sum per
 // value, each rounded to fp32 (no fused multiply-add), then one rounding to
 // bf16 or e4m3: the value does not depend on how the compiler contracts.
 // Values are turned in LDS: up to eight tokens of one dim are one store of
@@ -55,8 +56,8 @@ __device__ __forceinline__ void rotate8(const float* f, const float* cs, float* 
 
 constexpr int kEndsLds = 1024;  // sequence ends held in LDS for the search
 
-// RB rows x one head (blockIdx.y: query heads, key heads, value heads).
-template <int D, bool F8, int RB>
+// RB rows; blockIdx.y: groups of HB query and key heads, then value heads.
+template <int D, bool F8, int RB, int HB>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
   constexpr int V = D / 8, RP = 256 / V;        // vectors of a row, rows per pass
   constexpr int NP = RB > RP ? RB / RP : 1;     // passes
@@ -69,18 +70,22 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
 
   const int tid = threadIdx.x, c = tid % V, i0 = tid / V;
   const int64_t r0 = (int64_t)blockIdx.x * RB;
-  const int y = blockIdx.y;
-  const bool is_q = y < p.q_heads, is_v = y >= p.q_heads + p.kv_heads;
-  const int h = is_q ? y : (is_v ? y - p.q_heads - p.kv_heads : y - p.q_heads);
+  const int turned = p.q_heads + p.kv_heads, groups = (turned + HB - 1) / HB;
+  const bool is_v = (int)blockIdx.y >= groups;
+  const int y0 = is_v ? turned + (int)blockIdx.y - groups : (int)blockIdx.y * HB;
+  const int y1 = is_v ? y0 + 1 : (y0 + HB < turned ? y0 + HB : turned);
 
   bf16x8 x[NP];
+  auto load = [&](int y) {
 #pragma unroll
-  for (int u = 0; u < NP; ++u) {
-    const int i = i0 + RP * u;
-    x[u] = i < RB && r0 + i < p.b.n_rows
-               ? ld8(p.qkv + (r0 + i) * p.ld_qkv + (int64_t)y * D + 8 * c)
-               : zero8();
-  }
+    for (int u = 0; u < NP; ++u) {
+      const int i = i0 + RP * u;
+      x[u] = i < RB && r0 + i < p.b.n_rows
+                 ? ld8(p.qkv + (r0 + i) * p.ld_qkv + (int64_t)y * D + 8 * c)
+                 : zero8();
+    }
+  };
+  load(y0);
 
   const bool lds_ends = p.b.q_start && p.b.n_seqs <= kEndsLds;
   if (lds_ends) {
@@ -134,36 +139,59 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
   __syncthreads();
 
   if (!is_v) {
-    const float ks = F8 && !is_q ? p.k_scale[h] : 1.f;
+    float cs[NP][8];
+    int pos[NP], page[NP], slot[NP];
 #pragma unroll
     for (int u = 0; u < NP; ++u) {
       const int i = i0 + RP * u;
-      if (i >= RB) continue;
-      const int pos = sPos[i], page = sPage[i];
-      if (pos < 0 || (!is_q && page < 0)) continue;
-      const float* rp = p.rope + (int64_t)pos * D + 8 * c;
-      const f32x4_t ra = *(const f32x4_t*)rp, rb = *(const f32x4_t*)(rp + 4);
-      const float cs[8] = {ra[0], ra[1], ra[2], ra[3], rb[0], rb[1], rb[2], rb[3]};
-      float f[8], w[8];
-      unpack8(x[u], f);
-      rotate8(f, cs, w);
-      if (is_q) {
-        if (p.q_out) st8(p.q_out + (r0 + i) * p.ld_q + (int64_t)h * D + 8 * c, pack8(w));
-        continue;
+      pos[u] = i < RB ? sPos[i] : -1;
+      page[u] = i < RB ? sPage[i] : -1;
+      slot[u] = i < RB ? sSlot[i] : 0;
+      const float* rp = p.rope + (int64_t)(pos[u] < 0 ? 0 : pos[u]) * D + 8 * c;
+      f32x4_t a = f32x4_t{0.f, 0.f, 0.f, 0.f}, b = a;
+      if (pos[u] >= 0) {
+        a = *(const f32x4_t*)rp;
+        b = *(const f32x4_t*)(rp + 4);
       }
-      unsigned char* a =
-          p.k + ((((((int64_t)page * p.kv_heads + h) << p.b.lg_page) + sSlot[i]) * D) + 8 * c) * ES;
-      if constexpr (F8) {
-        uint2 o;
-        o.x = e4m3x4(w[0] / ks, w[1] / ks, w[2] / ks, w[3] / ks);
-        o.y = e4m3x4(w[4] / ks, w[5] / ks, w[6] / ks, w[7] / ks);
-        *(uint2*)a = o;
-      } else {
-        st8((bf16_t*)a, pack8(w));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        cs[u][e] = a[e];
+        cs[u][4 + e] = b[e];
+      }
+    }
+    for (int y = y0; y < y1; ++y) {
+      const bool is_q = y < p.q_heads;
+      const int h = is_q ? y : y - p.q_heads;
+      const float ks = F8 && !is_q ? p.k_scale[h] : 1.f;
+      bf16x8 now[NP];
+#pragma unroll
+      for (int u = 0; u < NP; ++u) now[u] = x[u];
+      if (y + 1 < y1) load(y + 1);
+#pragma unroll
+      for (int u = 0; u < NP; ++u) {
+        if (pos[u] < 0 || (!is_q && page[u] < 0)) continue;
+        float f[8], w[8];
+        unpack8(now[u], f);
+        rotate8(f, cs[u], w);
+        if (is_q) {
+          if (p.q_out) st8(p.q_out + (r0 + i0 + RP * u) * p.ld_q + (int64_t)h * D + 8 * c, pack8(w));
+          continue;
+        }
+        unsigned char* a =
+            p.k + ((((((int64_t)page[u] * p.kv_heads + h) << p.b.lg_page) + slot[u]) * D) + 8 * c) * ES;
+        if constexpr (F8) {
+          uint2 o;
+          o.x = e4m3x4(w[0] / ks, w[1] / ks, w[2] / ks, w[3] / ks);
+          o.y = e4m3x4(w[4] / ks, w[5] / ks, w[6] / ks, w[7] / ks);
+          *(uint2*)a = o;
+        } else {
+          st8((bf16_t*)a, pack8(w));
+        }
       }
     }
     return;
   }
+  const int h = y0 - turned;
 #pragma unroll
   for (int u = 0; u < NP; ++u) {
     const int i = i0 + RP * u;
@@ -204,18 +232,19 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
   }
 }
 
-template <int D, bool F8, int RB>
-static void launch_append_rows(const PagedAppend& p, int heads, hipStream_t s) {
-  const dim3 grid((unsigned)(((int64_t)p.b.n_rows + RB - 1) / RB), (unsigned)heads);
-  hipLaunchKernelGGL((paged_append_kernel<D, F8, RB>), grid, dim3(256), 0, s, p);
+template <int D, bool F8, int RB, int HB>
+static void launch_append_rows(const PagedAppend& p, hipStream_t s) {
+  const dim3 grid((unsigned)(((int64_t)p.b.n_rows + RB - 1) / RB),
+                  (unsigned)((p.q_heads + p.kv_heads + HB - 1) / HB + p.kv_heads));
+  hipLaunchKernelGGL((paged_append_kernel<D, F8, RB, HB>), grid, dim3(256), 0, s, p);
 }
 
 template <int D>
-static void launch_append(const PagedAppend& p, bool f8, bool small, int heads, hipStream_t s) {
-  if (f8 && small) launch_append_rows<D, true, 8>(p, heads, s);
-  else if (f8) launch_append_rows<D, true, 64>(p, heads, s);
-  else if (small) launch_append_rows<D, false, 8>(p, heads, s);
-  else launch_append_rows<D, false, 64>(p, heads, s);
+static void launch_append(const PagedAppend& p, bool f8, bool small, hipStream_t s) {
+  if (f8 && small) launch_append_rows<D, true, 8, 1>(p, s);
+  else if (f8) launch_append_rows<D, true, 64, 4>(p, s);
+  else if (small) launch_append_rows<D, false, 8, 1>(p, s);
+  else launch_append_rows<D, false, 64, 4>(p, s);
 }
 
 }  // namespace fvx
@@ -292,9 +321,9 @@ extern "C" int fvx_paged_append(const fvx_paged_append_desc* d, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   // few rows, or one per sequence (scattered value stores, one per token and
   // dim): many small workgroups
-  const bool small = !d->q_start || d->n_rows * heads < 64 * 256;
-  if (d->head_dim == 64) launch_append<64>(p, d->e4m3 != 0, small, heads, s);
-  else if (d->head_dim == 128) launch_append<128>(p, d->e4m3 != 0, small, heads, s);
-  else launch_append<256>(p, d->e4m3 != 0, small, heads, s);
+  const bool small = !d->q_start || d->n_rows * heads < 64 * 4 * 256;
+  if (d->head_dim == 64) launch_append<64>(p, d->e4m3 != 0, small, s);
+  else if (d->head_dim == 128) launch_append<128>(p, d->e4m3 != 0, small, s);
+  else launch_append<256>(p, d->e4m3 != 0, small, s);
   return launch_status("paged_append");
 }
