@@ -242,9 +242,9 @@ static void launch_append_rows(const PagedAppend& p, hipStream_t s) {
 template <int D>
 static void launch_append(const PagedAppend& p, bool f8, bool small, hipStream_t s) {
   if (f8 && small) launch_append_rows<D, true, 8, 1>(p, s);
-  else if (f8) launch_append_rows<D, true, 64, 4>(p, s);
+  else if (f8) launch_append_rows<D, true, 32, 8>(p, s);
   else if (small) launch_append_rows<D, false, 8, 1>(p, s);
-  else launch_append_rows<D, false, 64, 4>(p, s);
+  else launch_append_rows<D, false, 32, 8>(p, s);
 }
 
 }  // namespace fvx

@@ -613,9 +613,8 @@ __global__ __launch_bounds__(NT) void paged_merge_kernel(PagedAttn p) {
 // ---------------------------------------------------------------------------
 // Many rows per sequence: 32x32x16 MFMAs, keys and values through LDS
 // ---------------------------------------------------------------------------
-// Bound by the matrix cores and the exponentials.  A workgroup owns 128 NR
-// query rows of one key/value head, a wave 32 NR of them, and walks the keys
-// they see (or one of `splits` ranges of them) in tiles of 64.  Tiles arrive
+// Bound by the matrix cores and the exponentials.  A workgroup owns 128 query
+// rows of one key/value head, a wave 32 of them, and walks the keys they see (or one of `splits` ranges of them) in tiles of 64.  Tiles arrive
 // in LDS by DMA, one barrier per tile, keys one tile ahead of values.  A wave
 // goes on in halves of 32 keys, three of which are in work at once: the
 // scores of half h + 1 and the output of half h - 1 are on the matrix cores
@@ -694,8 +693,9 @@ __device__ __forceinline__ void mfma_settle() { asm volatile("s_nop 15\n\ts_nop 
 
 template <int D, bool F8>
 struct ProShape {
-  static constexpr int NR = 1;   // 32-row groups per wave
-  static constexpr int BM = 128 * NR;           // rows per workgroup
+  static constexpr int BM = 128;                // rows per workgroup
+  // workgroups per CU that registers and LDS allow
+  static constexpr int WGS = D == 256 ? 1 : (D == 128 ? 2 : 3);
   static constexpr int ES = F8 ? 1 : 2;
   static constexpr int KROW = D * ES;           // bytes of a key in LDS
   static constexpr int VROW = kProTile * ES;    // bytes of a dim in LDS
@@ -707,21 +707,19 @@ struct ProShape {
   // Products of a half: JA steps of the output, the scores' NC, the rest of
   // the output's NO.  Their operand fragments come from LDS in that order,
   // through a ring of registers, read kAhead fragments before their product.
-  // An output step is (block pair, step u, block, row group); e4m3 fragments
-  // hold both steps u of a block, or two steps of the scores.
+  // An output step is (block pair, step u, block); e4m3 fragments hold both steps u of a block, or two steps of the scores.
   static constexpr int NVR = F8 ? NDB : 2 * NDB;  // fragments of values
   static constexpr int NKR = F8 ? NS / 2 : NS;    // fragments of keys
-  static constexpr int NO = 2 * NDB * NR, NC = NS * NR, JA = NO / 2;
+  static constexpr int NO = 2 * NDB, NC = NS, JA = NO / 2;
   static constexpr int NVA = F8 && D == 64 ? NVR : NVR / 2;  // values' that the first JA use
   static constexpr int kRing = D == 64 ? 4 : 8, kAhead = D == 64 ? 3 : 6;
   // the output's fragment of its step j
   static constexpr int out_frag(int j) {
-    const int x = j / NR;
-    return F8 ? 2 * (x >> 2) + (x & 1) : x;
+    return F8 ? 2 * (j >> 2) + (j & 1) : j;
   }
   // the fragment, in reading order, of step j of a half
   static constexpr int frag_at(int j) {
-    if (j >= JA && j < JA + NC) return NVA + (j - JA) / NR / (F8 ? 2 : 1);
+    if (j >= JA && j < JA + NC) return NVA + (j - JA) / (F8 ? 2 : 1);
     const int r = out_frag(j < JA ? j : j - NC);
     return r < NVA ? r : r + NKR;
   }
@@ -804,9 +802,8 @@ __device__ bool find_tile(const PagedAttn& p, int item, int* scan, int* found, i
 }
 
 template <int D, bool F8, bool CAP>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(PagedAttn p) {
+__global__ __launch_bounds__(256, ProShape<D, F8>::WGS) void paged_prompt_kernel(PagedAttn p) {
   using S = ProShape<D, F8>;
-  constexpr int NR = S::NR;
   __shared__ __align__(16) unsigned char smem[4 * S::TB];
   __shared__ int sPid[kProPages];
   __shared__ int sScan[4], sFound[2], sMissing;
@@ -838,55 +835,55 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   }
 
   // this wave's rows: those past the tile's last repeat it and store nothing
-  const int r_wave = r_tile + 32 * NR * w;
-  const bool active = 32 * NR * w < rows;
-  int lo[NR], hi[NR], tok[NR], head[NR];
-  bf16x8 qf[NR][S::NS];
+  const int r_wave = r_tile + 32 * w;
+  const bool active = 32 * w < rows;
+  const int row = 32 * w + qi;  // of the tile
+  const int r = r_tile + (row < rows ? row : rows - 1);
+  const int tok = p.by_group.div(r), head = h * G + r - tok * G;
+  int lo, hi;
+  s.keys(p, tok, lo, hi);
+  bf16x8 qf[S::NS];
   // a negative scale turns the queries' signs (exact), a zero one clears
   // them: the scores' maximum can then be taken before scaling
   const float ks = F8 ? p.k_scale[h] : 1.f;
   const float raw = p.scale * ks;
   const float sc = (raw == 0.f ? 1.f : fabsf(raw)) * (CAP ? 2.f / p.softcap : 1.f) * kLog2e;
   const float cap = CAP ? p.softcap * kLog2e : 0.f;
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const int i = 32 * NR * w + 32 * n + qi;
-    const int r = r_tile + (i < rows ? i : rows - 1);
-    tok[n] = p.by_group.div(r);
-    head[n] = h * G + r - tok[n] * G;
-    s.keys(p, tok[n], lo[n], hi[n]);
-    const bf16_t* qr = p.q + (int64_t)(s.q0 + tok[n]) * p.ldq + (int64_t)head[n] * D;
+  {
+    const bf16_t* qr = p.q + (int64_t)(s.q0 + tok) * p.ldq + (int64_t)head * D;
 #pragma unroll
     for (int x = 0; x < S::NS; ++x) {
-      qf[n][x] = ld8(qr + (F8 ? 32 * (x >> 1) + 16 * hh + 8 * (x & 1) : 16 * x + 8 * hh));
+      qf[x] = ld8(qr + (F8 ? 32 * (x >> 1) + 16 * hh + 8 * (x & 1) : 16 * x + 8 * hh));
       if (raw <= 0.f)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) qf[n][x].w[e] = raw == 0.f ? 0u : qf[n][x].w[e] ^ 0x80008000u;
+        for (int e = 0; e < 4; ++e) qf[x].w[e] = raw == 0.f ? 0u : qf[x].w[e] ^ 0x80008000u;
     }
   }
+  // into accumulation registers here, two wait states or more before a product
+#pragma unroll
+  for (int x = 0; x < S::NS; ++x) {
+    i32x4_t v = __builtin_bit_cast(i32x4_t, qf[x]);
+    asm volatile("" : "+a"(v));
+    qf[x] = __builtin_bit_cast(bf16x8, v);
+  }
+  asm volatile("s_nop 1");
   // the wave's rows all see keys [lo_max, hi_min)
   int lo_max = lo_tile, hi_min = hi_tile;
   if (active) {
     int x;
-    const int last = r_wave + 32 * NR - 1 < r_tile + rows - 1 ? r_wave + 32 * NR - 1
-                                                              : r_tile + rows - 1;
+    const int last = min(r_wave + 31, r_tile + rows - 1);
     s.keys(p, p.by_group.div(r_wave), x, hi_min);
     s.keys(p, p.by_group.div(last), lo_max, x);
   }
 
   // O^T, the scores of a tile's halves (sa[half]) and their probabilities
-  f32x16_t o[NR][S::NDB], sa[2][NR];
-  bf16x8 pt[2][NR][2];
-  float ref[NR], l_run[NR];
+  f32x16_t o[S::NDB], sa[2];
+  bf16x8 pt[2][2];
+  float ref = -INFINITY, l_run = 0.f;
 #pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    ref[n] = -INFINITY;
-    l_run[n] = 0.f;
+  for (int db = 0; db < S::NDB; ++db)
 #pragma unroll
-    for (int db = 0; db < S::NDB; ++db)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[n][db][e] = 0.f;
-  }
+    for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
 
   // DMA: a wave brings 16 keys and D / 4 dims of a tile, LPW instructions of
   // 1 KiB each: RPK keys or RPV dims.  Its keys share a page.  A tile's
@@ -1005,20 +1002,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     const int ch = F8 ? 2 * hf + hh : 4 * hf + 2 * ((r >> 1) & 1) + hh;
     return *(const bf16x8*)(smem + (2 + (t & 1)) * S::TB + d * S::VROW + 16 * swz<S::VROW>(d, ch));
   };
-  auto out_step = [&](auto jc, const bf16x8& f, const bf16x8 (*pr)[2]) {
+  auto out_step = [&](auto jc, const bf16x8& f, const bf16x8* pr) {
     constexpr int j = decltype(jc)::value;
-    constexpr int n = j % NR, x = j / NR, pair = x >> 2, u = (x >> 1) & 1, db = 2 * pair + (x & 1);
+    constexpr int u = (j >> 1) & 1, db = 2 * (j >> 2) + (j & 1);
     if constexpr (F8)
-      mfma_output<true>(o[n][db], e4m3x8_to_bf16(f.w[2 * u], f.w[2 * u + 1]), pr[n][u]);
+      mfma_output<true>(o[db], e4m3x8_to_bf16(f.w[2 * u], f.w[2 * u + 1]), pr[u]);
     else
-      mfma_output<false>(o[n][db], f, pr[n][u]);
+      mfma_output<false>(o[db], f, pr[u]);
   };
-  auto score_step = [&](auto jc, const bf16x8& f, f32x16_t* d) {
-    constexpr int j = decltype(jc)::value, n = j % NR, x = j / NR;
+  auto score_step = [&](auto jc, const bf16x8& f, f32x16_t& d) {
+    constexpr int x = decltype(jc)::value;
     if constexpr (F8)
-      mfma_scores<x == 0, true>(d[n], e4m3x8_to_bf16(f.w[2 * (x & 1)], f.w[2 * (x & 1) + 1]), qf[n][x]);
+      mfma_scores<x == 0, true>(d, e4m3x8_to_bf16(f.w[2 * (x & 1)], f.w[2 * (x & 1) + 1]), qf[x]);
     else
-      mfma_scores<x == 0, false>(d[n], f, qf[n][x]);
+      mfma_scores<x == 0, false>(d, f, qf[x]);
   };
   auto capped = [&](float x) {  // in exponents of 2, of a score
     return cap - 2.f * cap * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * sc) + 1.f);
@@ -1032,9 +1029,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
   // maximum of the scores, the others over the exponentials.
   auto half = [&](int t, auto hfc) {
     constexpr int hf = decltype(hfc)::value;
-    f32x16_t* sv = sa[hf];
-    f32x16_t* sn = sa[hf ^ 1];
-    bf16x8 (*pr)[2] = pt[hf ^ 1];
+    f32x16_t& sv = sa[hf];
+    f32x16_t& sn = sa[hf ^ 1];
+    bf16x8* pr = pt[hf ^ 1];
     const int tv = hf ? t : t - 1, tk = hf ? t + 1 : t;
     bf16x8 ring[kRing];
     auto read = [&](auto rc) {
@@ -1059,89 +1056,77 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     };
     if (edge) {
       const uint32_t ok = there();
+      const uint32_t span = (uint32_t)(hi - lo), at = (uint32_t)(k0 - lo);
 #pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        const uint32_t span = (uint32_t)(hi[n] - lo[n]), at = (uint32_t)(k0 - lo[n]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const bool in = (at + (uint32_t)key_at(e) < span) & ((ok >> e & 1) != 0);
-          sv[n][e] = in ? sv[n][e] : -INFINITY;
-        }
+      for (int e = 0; e < 16; ++e) {
+        const bool in = (at + (uint32_t)key_at(e) < span) & ((ok >> e & 1) != 0);
+        sv[e] = in ? sv[e] : -INFINITY;
       }
     }
 
-    constexpr int JB = NO - JA + NC, NE = 16 * NR;
-    float mx[NR];
+    constexpr int JB = NO - JA + NC;
+    float mx;
     static_for<0, JA>([&](auto jc) {
       constexpr int j = decltype(jc)::value;
       static_for<j ? kAhead + S::frags_to(j - 1) : kAhead, kAhead + S::frags_to(j)>([&](auto rc) { read(rc); });
       out_step(jc, ring[S::frag_at(j) % kRing], pr);
-      static_for<NE * j / JA, NE * (j + 1) / JA>([&](auto qc) {
-        constexpr int q = decltype(qc)::value, n = q / 16, e = q % 16;
-        if constexpr (e % 2 == 1) mx[n] = max3(e == 1 ? sv[n][0] : mx[n], sv[n][e - 1], sv[n][e]);
-        if constexpr (e % 2 == 1) l_run[n] = add_pair(pr[n][e >> 3].w[(e & 7) >> 1], l_run[n]);
+      static_for<8 * j / JA, 8 * (j + 1) / JA>([&](auto qc) {
+        constexpr int q = decltype(qc)::value, e = 2 * q;
+        mx = max3(q == 0 ? sv[0] : mx, sv[e], sv[e + 1]);
+        l_run = add_pair(pr[q >> 2].w[q & 3], l_run);
       });
       __builtin_amdgcn_sched_barrier(0);
     });
-    bool up = false;
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      float m = half_pair_max(mx[n]);
-      mx[n] = m == -INFINITY ? m : (CAP ? capped(m) : m * sc);
-      up = up || mx[n] > ref[n] + kSlack;
-    }
-    if (__any(up)) {
+    mx = half_pair_max(mx);
+    if (mx != -INFINITY) mx = CAP ? capped(mx) : mx * sc;
+    if (__any(mx > ref + kSlack)) {
       // the probabilities not yet in the output follow it to the new
       // reference (a second rounding to bf16, on the halves where it rises)
       mfma_settle();
+      const float nr = fmaxf(ref, mx);
+      const float f = ref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - nr);
+      ref = nr;
+      l_run *= f;
 #pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        const float nr = fmaxf(ref[n], mx[n]);
-        const float f = ref[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref[n] - nr);
-        ref[n] = nr;
-        l_run[n] *= f;
+      for (int db = 0; db < S::NDB; ++db) {
+        asm volatile("" : "+a"(o[db]));  // not copied before it is settled
 #pragma unroll
-        for (int db = 0; db < S::NDB; ++db) {
-          asm volatile("" : "+a"(o[n][db]));  // not copied before it is settled
+        for (int e = 0; e < 16; ++e) o[db][e] *= f;
+        asm volatile("" : "+a"(o[db]));  // and back before the paths join
+      }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[n][db][e] *= f;
-          asm volatile("" : "+a"(o[n][db]));  // and back before the paths join
-        }
+      for (int u = 0; u < 2; ++u) {
+        float x[8];
+        unpack8(pr[u], x);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float x[8];
-          unpack8(pr[n][u], x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= f;
-          pr[n][u] = pack8(x);
-        }
+        for (int e = 0; e < 8; ++e) x[e] *= f;
+        pr[u] = pack8(x);
       }
     }
-    float nm[NR], even = 0.f;
-#pragma unroll
-    for (int n = 0; n < NR; ++n) nm[n] = (CAP ? cap : 0.f) - (ref[n] == -INFINITY ? 0.f : ref[n]);
+    const float nm = (CAP ? cap : 0.f) - (ref == -INFINITY ? 0.f : ref);
+    float even = 0.f;
     static_for<0, JB>([&](auto jc) {
       constexpr int j = JA + decltype(jc)::value, jb = decltype(jc)::value;
       static_for<kAhead + S::frags_to(j - 1), kAhead + S::frags_to(j)>([&](auto rc) { read(rc); });
       const bf16x8& f = ring[S::frag_at(j) % kRing];
       if constexpr (jb < NC) score_step(IntC<jb>{}, f, sn);
       else out_step(IntC<j - NC>{}, f, pr);
-      static_for<NE * jb / JB, NE * (jb + 1) / JB>([&](auto qc) {
-        constexpr int q = decltype(qc)::value, n = q / 16, e = q % 16;
-        const float x = sv[n][e];
+      static_for<16 * jb / JB, 16 * (jb + 1) / JB>([&](auto ec) {
+        constexpr int e = decltype(ec)::value;
+        const float x = sv[e];
         float pv;
         if constexpr (CAP) {
           const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * sc) + 1.f);
-          pv = __builtin_amdgcn_exp2f(fmaf(-2.f * cap, r, nm[n]));
+          pv = __builtin_amdgcn_exp2f(fmaf(-2.f * cap, r, nm));
         } else {
-          pv = __builtin_amdgcn_exp2f(fmaf(x, sc, nm[n]));
+          pv = __builtin_amdgcn_exp2f(fmaf(x, sc, nm));
         }
         if constexpr (e % 2 == 0) {
           even = pv;
         } else {
           uint32_t w2 = f2bf2(even, pv);
           asm volatile("" : "+v"(w2));  // here, under the products, not behind them
-          pt[hf][n][e >> 3].w[(e & 7) >> 1] = w2;
+          pt[hf][e >> 3].w[(e & 7) >> 1] = w2;
         }
       });
       __builtin_amdgcn_sched_barrier(0);
@@ -1149,11 +1134,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     // (a capped score of minus infinity is minus the cap)
     if (CAP && edge) {
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          pt[hf][n][e >> 3].w[(e & 7) >> 1] &=
-              sv[n][e] == -INFINITY ? (e & 1 ? 0xffffu : 0xffff0000u) : 0xffffffffu;
+      for (int e = 0; e < 16; ++e)
+        pt[hf][e >> 3].w[(e & 7) >> 1] &=
+            sv[e] == -INFINITY ? (e & 1 ? 0xffffu : 0xffff0000u) : 0xffffffffu;
     }
   };
 
@@ -1163,12 +1146,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     if (tid == 0) sMissing = 0;
     __syncthreads();
     fill_ids(run0);
-    fill_ids(run0 + kProRun);
+    if (t1 > run0 + kProRun) fill_ids(run0 + kProRun);
     // the first half's "previous" values: zeros (with zero probabilities)
     for (int i = tid; i < S::TB / 16; i += 256)
       *(bf16x8*)(smem + (2 + ((t0 + 1) & 1)) * S::TB + 16 * i) = zero8();
-#pragma unroll
-    for (int n = 0; n < NR; ++n) pt[1][n][0] = pt[1][n][1] = zero8();
+    pt[1][0] = pt[1][1] = zero8();
     __syncthreads();
     {
       const Ids d = fetch_ids(t0, t0);
@@ -1189,7 +1171,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     auto turn = [&](int t, const Ids& d) {
       wait_vmcnt<0>();
       clear_v(t);
-      if ((t & (kProRun - 1)) == 2 && t - 2 > run0) fill_ids(t - 2 + kProRun);
+      if ((t & (kProRun - 1)) == 2 && t - 2 > run0 && t - 2 + kProRun < t1)
+        fill_ids(t - 2 + kProRun);
       // (a run's pages are looked up a hundred tiles before they are used)
       missing = __builtin_amdgcn_readfirstlane(d.none) != 0;
       __syncthreads();
@@ -1203,7 +1186,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     } else {
       static_for<0, NC>([&](auto jc) {
         constexpr int j = decltype(jc)::value;
-        score_step(jc, read_k(t0, 0, j / (F8 ? 2 * NR : NR)), sa[0]);
+        score_step(jc, read_k(t0, 0, j / (F8 ? 2 : 1)), sa[0]);
       });
       mfma_settle();
       for (int t = t0; t < t1; ++t) {
@@ -1213,9 +1196,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
         half(t, IntC<1>{});
       }
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) l_run[n] = add_pair(pt[1][n][e >> 2].w[e & 3], l_run[n]);
+      for (int e = 0; e < 8; ++e) l_run = add_pair(pt[1][e >> 2].w[e & 3], l_run);
       static_for<0, NO>([&](auto jc) {
         out_step(jc, read_v(t1 - 1, 1, S::out_frag(decltype(jc)::value)), pt[1]);
       });
@@ -1232,39 +1213,34 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_prompt_kernel(Pag
     p.prec[prob * 4 + 2] = r_tile;
     p.prec[prob * 4 + 3] = h;
   }
+  const float l = half_pair_sum(l_run);
 #pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const int i = 32 * NR * w + 32 * n + qi;
-    const float l = half_pair_sum(l_run[n]);
+  for (int db = 0; db < S::NDB; ++db) asm volatile("" : "+a"(o[db]));
+  if (row >= rows) return;
+  if (p.splits == 1) {
+    const float inv = l > 0.f ? vs / l : 0.f;
+    bf16_t* out = p.o + (int64_t)(s.q0 + tok) * p.ldo + (int64_t)head * D + 4 * hh;
 #pragma unroll
-    for (int db = 0; db < S::NDB; ++db) asm volatile("" : "+a"(o[n][db]));
-    if (i >= rows) continue;
-    if (p.splits == 1) {
-      const float inv = l > 0.f ? vs / l : 0.f;
-      bf16_t* row = p.o + (int64_t)(s.q0 + tok[n]) * p.ldo + (int64_t)head[n] * D + 4 * hh;
+    for (int db = 0; db < S::NDB; ++db)
 #pragma unroll
-      for (int db = 0; db < S::NDB; ++db)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint2 v;
-          v.x = f2bf2(o[n][db][4 * j] * inv, o[n][db][4 * j + 1] * inv);
-          v.y = f2bf2(o[n][db][4 * j + 2] * inv, o[n][db][4 * j + 3] * inv);
-          *(uint2*)(row + 32 * db + 8 * j) = v;
-        }
-    } else {
-      float* row = part + i * D + 4 * hh;
-#pragma unroll
-      for (int db = 0; db < S::NDB; ++db)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *(f32x4_t*)(row + 32 * db + 8 * j) =
-              f32x4_t{o[n][db][4 * j] * vs, o[n][db][4 * j + 1] * vs, o[n][db][4 * j + 2] * vs,
-                      o[n][db][4 * j + 3] * vs};
-      if (hh == 0) {
-        part[S::BM * D + i] = ref[n];
-        part[S::BM * D + S::BM + i] = l;
+      for (int j = 0; j < 4; ++j) {
+        uint2 v;
+        v.x = f2bf2(o[db][4 * j] * inv, o[db][4 * j + 1] * inv);
+        v.y = f2bf2(o[db][4 * j + 2] * inv, o[db][4 * j + 3] * inv);
+        *(uint2*)(out + 32 * db + 8 * j) = v;
       }
-    }
+    return;
+  }
+  float* out = part + row * D + 4 * hh;
+#pragma unroll
+  for (int db = 0; db < S::NDB; ++db)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *(f32x4_t*)(out + 32 * db + 8 * j) = f32x4_t{o[db][4 * j] * vs, o[db][4 * j + 1] * vs,
+                                                   o[db][4 * j + 2] * vs, o[db][4 * j + 3] * vs};
+  if (hh == 0) {
+    part[S::BM * D + row] = ref;
+    part[S::BM * D + S::BM + row] = l;
   }
 }
 
@@ -1358,13 +1334,16 @@ static PagedPlan paged_plan(const fvx_paged_attn_desc* d) {
   a.prec = a.part + (int64_t)a.n_wg * 2 * kDecRows * (d->head_dim + 2) * 4;
   a.ppart = a.bytes = a.prec;
   if (a.many) {
-    const int64_t bm = 128;
+    constexpr int64_t bm = ProShape<64, false>::BM;  // of any
     a.problems = (d->n_rows * G / bm + (d->n_seqs < d->n_rows ? d->n_seqs : d->n_rows)) * d->kv_heads;
     // With fewer problems than workgroups that run at once their keys are
     // split, no finer than tiles of 64 keys and into 64 ranges at most, whose
     // partials cost as much as they save (one sequence of 4000 keys, 40 rows
     // of 256 dims: 62 us in 128 ranges).
-    const int64_t at_once = device_cus() * (d->head_dim == 256 ? 1 : 2);
+    const int64_t at_once =
+        device_cus() * (d->head_dim == 256 ? ProShape<256, false>::WGS
+                                           : (d->head_dim == 128 ? ProShape<128, false>::WGS
+                                                                 : ProShape<64, false>::WGS));
     const int64_t tiles = (d->max_pages * d->page_size + 63) / 64;
     int64_t s = at_once / a.problems;
     s = s < 64 ? s : 64;
