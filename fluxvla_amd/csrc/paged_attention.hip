@@ -802,7 +802,7 @@ __device__ bool find_tile(const PagedAttn& p, int item, int* scan, int* found, i
 }
 
 template <int D, bool F8, bool CAP>
-__global__ __launch_bounds__(256, ProShape<D, F8>::WGS) void paged_prompt_kernel(PagedAttn p) {
+__global__ __launch_bounds__(256, (ProShape<D, F8>::WGS)) void paged_prompt_kernel(PagedAttn p) {
   using S = ProShape<D, F8>;
   __shared__ __align__(16) unsigned char smem[4 * S::TB];
   __shared__ int sPid[kProPages];
