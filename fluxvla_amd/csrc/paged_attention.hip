@@ -756,30 +756,36 @@ __device__ bool find_tile(const PagedAttn& p, int item, int* scan, int* found, i
     const int64_t rows = (int64_t)n * p.group;
     return rows > p.most_rows ? (int)((rows + BM - 1) / BM) : 0;
   };
-  int mine = 0;  // (problems are fewer than 2^31)
+  // Starts that run backwards make sequences overlap: sums that saturate keep
+  // every problem of the launch in the one run [at, incl) that holds it.
+  int mine = 0;
   for (int i = 0; i < each; ++i)
-    if (first + i < p.b.n_seqs) mine += tiles(first + i);
+    if (first + i < p.b.n_seqs) mine = __builtin_elementwise_add_sat(mine, tiles(first + i));
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int v = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += v;
+    if (lane >= o) incl = __builtin_elementwise_add_sat(incl, v);
   }
-  int at = incl - mine, total = __builtin_amdgcn_readlane(incl, 63);
+  int at = __shfl_up(incl, 1, 64), total = __builtin_amdgcn_readlane(incl, 63);
+  if (lane == 0) at = 0;
   if (!lanes) {
     if (lane == 63) scan[wave] = incl;
     __syncthreads();
     total = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (i < wave) at += scan[i];
-      total += scan[i];
+      if (i < wave) {
+        at = __builtin_elementwise_add_sat(at, scan[i]);
+        incl = __builtin_elementwise_add_sat(incl, scan[i]);
+      }
+      total = __builtin_elementwise_add_sat(total, scan[i]);
     }
   }
   const int want = p.by_kv.div(item);
   h = item - want * p.kv_heads;
   if (want >= total) return false;
-  const bool here = want >= at && want < at + mine;
+  const bool here = want >= at && want < incl;
   if (lanes) {
     b = __builtin_ctzll(__ballot(here));
     t = __builtin_amdgcn_readlane(mine - 1 - (want - at), b);
@@ -789,7 +795,7 @@ __device__ bool find_tile(const PagedAttn& p, int item, int* scan, int* found, i
     int s = first, n;
     for (;; ++s) {
       n = tiles(s);
-      if (want < at + n) break;
+      if (want - at < n) break;
       at += n;
     }
     found[0] = s;

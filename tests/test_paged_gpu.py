@@ -249,6 +249,27 @@ def test_equal_prompts_need_no_workspace(cuda):
     _attend(cuda, [20 + i for i in range(16)], [20] * 16, 16, 16, 64, 16)
 
 
+def test_overlapping_starts_of_many_sequences(cuda):
+    # starts that run backwards: rows of several sequences, in any of their
+    # values, and nothing outside the rows
+    announce('paged overlapping starts')
+    cache = K.PagedKV(torch.zeros(4, 1, 16, 64, dtype=torch.bfloat16, device=cuda),
+                      torch.ones(4, 1, 64, 16, dtype=torch.bfloat16, device=cuda))
+    n, rows = 200, 300
+    starts = torch.tensor([0, 250] * (n // 2) + [0], dtype=torch.int32, device=cuda)
+    table = torch.arange(4, dtype=torch.int32, device=cuda).repeat(n, 1)
+    lens = torch.full((n,), 60, dtype=torch.int32, device=cuda)
+    full = torch.full((rows + 2, 2, 64), 7.0, dtype=torch.bfloat16, device=cuda)
+    q = torch.ones(rows, 2, 64, dtype=torch.bfloat16, device=cuda)
+    for most in (0, 8, 250):
+        K.paged_attention(q, cache, table, lens, out=full[1:-1], q_start=starts, max_q=most)
+        torch.cuda.synchronize()
+        out = full.float()
+        assert (out[0] == 7).all() and (out[251:] == 7).all()
+        # the rows before a sequence's start see nothing, the others ones
+        assert (((out[1:251] - 1).abs() <= 2 ** -7) | (out[1:251] == 0) | (out[1:251] == 7)).all()
+
+
 def test_more_new_tokens_than_length(cuda):
     # the first rows lie before the sequence's start: they see nothing
     announce('paged prompt rows before the start')
