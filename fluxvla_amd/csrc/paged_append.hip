@@ -268,11 +268,11 @@ extern "C" int fvx_paged_append(const fvx_paged_append_desc* d, void* stream) {
               "paged_append: kv_heads (> 0) and q_heads (>= 0) out of range: %lld, %lld",
               (long long)d->kv_heads, (long long)d->q_heads);
   const int64_t big = 1ll << 30;
-  FVX_REQUIRE(d->n_rows < big && d->n_seqs < big && d->n_pages > 0 && d->n_pages < 2 * big &&
+  FVX_REQUIRE(d->n_rows < big / 16 && d->n_seqs < big && d->n_pages > 0 && d->n_pages < 2 * big &&
                   d->max_pages < big && d->max_pages * d->page_size < big && d->max_pos < 2 * big,
               FVX_ERR_SHAPE,
-              "paged_append: n_rows, n_seqs and max_pages * page_size must be below 2^30, "
-              "n_pages (> 0) and max_pos below 2^31");
+              "paged_append: n_rows must be below 2^26, n_seqs and max_pages * page_size below "
+              "2^30, n_pages (> 0) and max_pos below 2^31");
   FVX_REQUIRE(d->q_start || d->n_rows == d->n_seqs, FVX_ERR_SHAPE,
               "paged_append: without q_start n_rows (%lld) must be n_seqs (%lld)",
               (long long)d->n_rows, (long long)d->n_seqs);

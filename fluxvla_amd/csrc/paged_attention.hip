@@ -1426,7 +1426,15 @@ static int check_paged_attention(const fvx_paged_attn_desc* d) {
               (long long)d->n_rows, (long long)d->n_seqs);
   FVX_REQUIRE(d->e4m3 == 0 || d->e4m3 == 1, FVX_ERR_ARG, "paged_attention: e4m3 must be 0 or 1");
   FVX_REQUIRE(d->softcap >= 0.f && isfinite(d->softcap) && isfinite(d->scale), FVX_ERR_ARG,
-              "paged_attention: scale must be finite, softcap finite and >= 0");
+              "paged_attention: scale and softcap must be finite, softcap >= 0");
+  // cap(x) is formed as softcap (1 - 2 / (exp(2 x / softcap) + 1)), which
+  // costs a score 3 * 2^-24 softcap: 2e-4 at most
+  FVX_REQUIRE(d->softcap <= 1024.f, FVX_ERR_ARG, "paged_attention: softcap=%g must be at most 1024",
+              (double)d->softcap);
+  const float per_cap = d->softcap > 0.f ? 2.f * kLog2e / d->softcap : 0.f;
+  FVX_REQUIRE(isfinite(per_cap) && isfinite(per_cap * d->scale), FVX_ERR_ARG,
+              "paged_attention: softcap=%g is too small for scale=%g", (double)d->softcap,
+              (double)d->scale);
   return FVX_OK;
 }
 
@@ -1462,8 +1470,9 @@ extern "C" int fvx_paged_attention(const fvx_paged_attn_desc* d, void* stream) {
               "paged_attention: ldq and ldo must hold q_heads * head_dim values, table_stride "
               "max_pages entries");
   const PagedPlan plan = paged_plan(d);
-  FVX_REQUIRE(plan.problems < 1ll << 31, FVX_ERR_SHAPE,
-              "paged_attention: too many rows and sequences for one launch");
+  FVX_REQUIRE(plan.problems < 1ll << 24, FVX_ERR_SHAPE,
+              "paged_attention: (n_rows * q_heads / kv_heads / 128 + n_seqs) * kv_heads must be "
+              "below 2^24");
   FVX_REQUIRE(plan.bytes == 0 || (d->workspace && d->workspace_bytes >= plan.bytes),
               FVX_ERR_WORKSPACE,
               "paged_attention: workspace of %lld bytes required", (long long)plan.bytes);

@@ -997,7 +997,9 @@ def paged_attention(q, cache, page_table, kv_len, out=None, q_start=None,
     A token at position t sees keys j <= t, all keys j < prefix_len[b]
     (int32 [n_seqs]) and, with ``window``, only keys j > t - window.
     ``softcap`` c > 0: scores c * tanh(s / c).  A token that sees nothing
-    gives zeros; rows behind the last sequence are left as they were.
+    gives zeros; rows behind the last sequence are left as they were.  Slots
+    that no new token of a sequence sees may hold anything; a value that
+    only some of them see must be finite.  ``softcap`` is at most 1024.
     ``max_q``: the most new tokens of one sequence when known (a hint).
     ``workspace``: uint8 [paged_attention_workspace_bytes], taken from the
     allocator unless given; calls on different streams need their own."""

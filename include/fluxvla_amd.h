@@ -757,13 +757,21 @@ int fvx_paged_append(const fvx_paged_append_desc* d, void* stream);
  * j <= t or j < prefix_len[b] (NULL: 0) and, with window > 0, j > t - window.
  * A row that sees no key (a position before the sequence's start, missing
  * pages) is zero; rows that belong to no sequence are left as they were.
- * What unwritten slots hold does not matter, infinities and NaN included.
+ * What slots hold that no new row of a sequence sees does not matter,
+ * infinities and NaN included; a value that some rows see and others do not
+ * (a later token's, one that leaves the window) must be finite, or it reaches
+ * those too (with weight zero).
  * fp32 scores, statistics and sums; bf16 probabilities in the second product.
  * max_q: a hint, the most rows of a sequence (0: unknown); any value gives
  * the same sums, in an order that may differ.
  * workspace: fvx_paged_attention_workspace_bytes(d) bytes, 16-byte aligned,
  * of any contents; nothing in it is kept between calls, but calls that overlap
- * (other streams) need workspaces of their own.
+ * (other streams) need workspaces of their own.  They depend on the sizes
+ * (n_rows, n_seqs, max_pages, page_size, heads, head_dim, max_q) and on whether
+ * q_start is given; none may be needed (0, workspace NULL).
+ * Limits: softcap 1024; q_heads 4096; (n_rows * q_heads / kv_heads / 128 +
+ * n_seqs) * kv_heads below 2^24 for rows that are not single tokens of up to
+ * 16 heads per key/value head; fvx_paged_append: n_rows below 2^26.
  */
 typedef struct fvx_paged_attn_desc {
   const void* q; int64_t ldq;      /* [n_rows][q_heads][head_dim] bf16 */

@@ -85,6 +85,7 @@ BOTH = [
     ({'ld_qkv': 2552}, _lib.FVX_ERR_SHAPE, 'ld_qkv'),
     ({'ld_q': 2040}, _lib.FVX_ERR_SHAPE, 'ld_q'),
     ({'max_pos': -1}, _lib.FVX_ERR_SHAPE, 'max_pos'),
+    ({'n_rows': 1 << 26, 'n_seqs': 1 << 26}, _lib.FVX_ERR_SHAPE, '2^26'),
 ])
 def test_append_refuses(kw, status, text):
     lib = _lib.load()
@@ -100,6 +101,8 @@ def test_append_refuses(kw, status, text):
     ({'softcap': -1.0}, _lib.FVX_ERR_ARG, 'softcap'),
     ({'softcap': float('inf')}, _lib.FVX_ERR_ARG, 'softcap'),
     ({'scale': float('nan')}, _lib.FVX_ERR_ARG, 'scale'),
+    ({'softcap': 1e-39}, _lib.FVX_ERR_ARG, 'too small'),
+    ({'softcap': 1025.0}, _lib.FVX_ERR_ARG, '1024'),
     ({'ldq': 2044}, _lib.FVX_ERR_ALIGN, 'multiples of 8'),
     ({'ldo': 2040}, _lib.FVX_ERR_SHAPE, 'ldo'),
     ({}, _lib.FVX_ERR_WORKSPACE, 'workspace'),

@@ -249,6 +249,66 @@ def test_equal_prompts_need_no_workspace(cuda):
     _attend(cuda, [20 + i for i in range(16)], [20] * 16, 16, 16, 64, 16)
 
 
+@pytest.mark.parametrize('e4m3', [False, True])
+@pytest.mark.parametrize('kw', [{}, {'window': 9000}, {'window': 300}])
+def test_one_workgroup_walks_a_long_sequence(cuda, e4m3, kw):
+    # so many sequences that keys are not split: one workgroup goes through
+    # 20000 keys, page ids in runs, a page missing in the last run
+    def edit(table, k, v):
+        table[0, 1230] = -1
+    announce(f'paged prompt long walk e4m3={e4m3} {kw}')
+    lens = [20000] + [i % 7 + 1 for i in range(1, 800)]
+    _attend(cuda, lens, [20] + [1] * 799, 1, 1, 64, 16, e4m3, edit=edit, single=False, **kw)
+
+
+def test_workgroups_walk_more_pages_than_they_hold(cuda):
+    # 64 sequences over the same 4375 pages of 16 tokens: 547 blocks of keys
+    # for each workgroup of the single-token kernel
+    announce('paged decode long walk over shared pages')
+    n, d, seqs = 70000, 64, 64
+    k, v, _, _, table = _pool([n], 1, d, 16, False, 12)
+    q = torch.randn(seqs, 2, d, generator=torch.Generator().manual_seed(2)).bfloat16()
+    lens = [n - 13 * i for i in range(seqs)]
+    out = K.paged_attention(q.to(cuda), K.PagedKV(k.to(cuda), v.to(cuda)),
+                            table.repeat(seqs, 1).to(cuda),
+                            torch.tensor(lens, dtype=torch.int32, device=cuda))
+    use = table[0, :n // 16].long()
+    kk = k[use, 0].double().reshape(-1, d)
+    vv = v[use, 0].double().transpose(1, 2).reshape(-1, d)
+    for b in (0, 31, 63):
+        p = torch.softmax(q[b].double() @ kk[:lens[b]].t() * d ** -0.5, -1)
+        _close(out[b], p @ vv[:lens[b]], p @ vv[:lens[b]].abs())
+
+
+@pytest.mark.parametrize('new', [[1, 1], [40, 7]])
+@pytest.mark.parametrize('scale', [-0.2, 0.0])
+@pytest.mark.parametrize('softcap', [0.0, 10.0])
+def test_negative_and_zero_scales(cuda, new, scale, softcap):
+    announce(f'paged scale={scale} softcap={softcap} new={new}')
+    _attend(cuda, [80, 40], new, 4, 2, 64, 16, scale=scale, softcap=softcap,
+            fill=float('nan'))
+
+
+@pytest.mark.parametrize('new', [[1, 1], [3, 5], [40, 7]])
+@pytest.mark.parametrize('softcap', [0.01, 1024.0])
+def test_extreme_caps(cuda, new, softcap):
+    # scores lose 3 * 2^-24 * 1024 * log2(e) * ln(2) = 2e-4 < 2^-10 to a cap of 1024
+    announce(f'paged softcap={softcap} new={new}')
+    _attend(cuda, [80, 40], new, 4, 2, 64, 16, softcap=softcap)
+
+
+@pytest.mark.parametrize('most', [1, 4, 60])
+@pytest.mark.parametrize('kw', [{'window': 33}, {'prefix': True}, {'softcap': 20.0}])
+def test_more_sequences_than_lanes(cuda, most, kw):
+    announce(f'paged 70 sequences most={most} {kw}')
+    new = [1] * 70 if most == 1 else [i % (most + 1) for i in range(70)]
+    lens = [n + (11 * i) % 190 for i, n in enumerate(new)]
+    kw = dict(kw)
+    if 'prefix' in kw:
+        kw['prefix'] = [7 * i % 150 for i in range(70)]
+    _attend(cuda, lens, new, 4, 2, 64, 16, **kw)
+
+
 def test_overlapping_starts_of_many_sequences(cuda):
     # starts that run backwards: rows of several sequences, in any of their
     # values, and nothing outside the rows
@@ -268,6 +328,78 @@ def test_overlapping_starts_of_many_sequences(cuda):
         assert (out[0] == 7).all() and (out[251:] == 7).all()
         # the rows before a sequence's start see nothing, the others ones
         assert (((out[1:251] - 1).abs() <= 2 ** -7) | (out[1:251] == 0) | (out[1:251] == 7)).all()
+
+
+def test_two_graphs_of_different_calls(cuda):
+    announce('paged two graphs')
+    k, v, _, _, table = _pool([900, 700], 1, 64, 16, False, 14)
+    cache, t = K.PagedKV(k.to(cuda), v.to(cuda)), table.to(cuda)
+    lens = torch.tensor([900, 700], dtype=torch.int32, device=cuda)
+    starts = _starts([30, 2]).to(cuda)
+    g = torch.Generator().manual_seed(6)
+    q1 = torch.randn(2, 8, 64, generator=g).bfloat16().to(cuda)
+    q2 = torch.randn(32, 8, 64, generator=g).bfloat16().to(cuda)
+
+    def one():
+        return K.paged_attention(q1, cache, t, lens)
+
+    def many():
+        return K.paged_attention(q2, cache, t, lens, q_start=starts, max_q=30)
+
+    one(), many()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for f in (one, many):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(f())
+    for n in ([900, 700], [17, 650], [1, 0], [900, 32]):
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        for gr in (graphs[0], graphs[1], graphs[0]):
+            gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], one()) and torch.equal(outs[1], many())
+
+
+def test_empty_calls(cuda):
+    announce('paged empty calls')
+    cache = K.PagedKV.empty(2, 16, 1, 64, cuda)
+    table = torch.zeros(0, 3, dtype=torch.int32, device=cuda)
+    none = torch.zeros(0, dtype=torch.int32, device=cuda)
+    out = K.paged_attention(torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=cuda), cache, table,
+                            none)
+    assert out.shape == (0, 4, 64)
+    # rows, but no sequence: they stay
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=cuda)
+    out = torch.full_like(q, 5.0)
+    start = torch.zeros(1, dtype=torch.int32, device=cuda)
+    K.paged_attention(q, cache, table, none, out=out, q_start=start)
+    assert (out == 5.0).all()
+    # a table without pages: nothing to see, nowhere to write
+    table = torch.zeros(2, 0, dtype=torch.int32, device=cuda)
+    lens = torch.tensor([3, 4], dtype=torch.int32, device=cuda)
+    assert (K.paged_attention(q[:2], cache, table, lens) == 0).all()
+    before = cache.k.clone()
+    got = K.paged_append(torch.ones(2, 6 * 64, dtype=torch.bfloat16, device=cuda), cache,
+                         K.rope_table(4, 64, device=cuda), table, lens, 4)
+    assert torch.isfinite(got.float()).all() and torch.equal(cache.k.view(torch.int16),
+                                                             before.view(torch.int16))
+
+
+def test_workspace_bytes_are_enough(cuda):
+    announce('paged workspace bytes')
+    for new in ([1, 1], [5, 3], [200, 1]):
+        lens = [900, 300]
+        k, v, _, _, table = _pool(lens, 1, 64, 16, False, 13)
+        cache, t = K.PagedKV(k.to(cuda), v.to(cuda)), table.to(cuda)
+        q = torch.randn(sum(new), 8, 64, generator=torch.Generator().manual_seed(3)).bfloat16().to(cuda)
+        ln = torch.tensor(lens, dtype=torch.int32, device=cuda)
+        st = None if max(new) == 1 else _starts(new).to(cuda)
+        n = K.paged_attention_workspace_bytes(q, cache, t, st, max(new))
+        ws = torch.full((n + 64,), 0x55, dtype=torch.uint8, device=cuda)
+        got = K.paged_attention(q, cache, t, ln, q_start=st, max_q=max(new), workspace=ws[:n])
+        assert torch.equal(got, K.paged_attention(q, cache, t, ln, q_start=st, max_q=max(new)))
+        assert (ws[n:] == 0x55).all()
 
 
 def test_more_new_tokens_than_length(cuda):
