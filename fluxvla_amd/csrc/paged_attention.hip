@@ -105,7 +105,10 @@ struct PagedSeq {
 // ---------------------------------------------------------------------------
 // Few rows per sequence: up to 16 rows a problem on 16x16x32 MFMAs
 // ---------------------------------------------------------------------------
-// Bound by the cache's bytes.  All (sequence, key/value head, 16 rows)
+// Bound by the cache's bytes: 64 sequences of 1 to 8192 tokens, 32 heads on 8
+// of 128 dims, 1.07 GB: 185 us + 5 of the merge, 5.6 TB/s where reading alone
+// reaches 5.7; short caches by a chain of dependent loads (817 tokens: 7 us
+// and 3.3).  All (sequence, key/value head, 16 rows)
 // problems form one line of units, a key block each, which is cut evenly
 // over the workgroups, one per CU: lengths may differ as they like, and the
 // host need not know them.  A workgroup walks its piece problem by problem,
@@ -613,9 +616,15 @@ __global__ __launch_bounds__(NT) void paged_merge_kernel(PagedAttn p) {
 // ---------------------------------------------------------------------------
 // Many rows per sequence: 32x32x16 MFMAs, keys and values through LDS
 // ---------------------------------------------------------------------------
-// Bound by the matrix cores and the exponentials.  A workgroup owns 128 query
-// rows of one key/value head, a wave 32 of them, and walks the keys they see (or one of `splits` ranges of them) in tiles of 64.  Tiles arrive
-// in LDS by DMA, one barrier per tile, keys one tile ahead of values.  A wave
+// Bound by what a SIMD issues: products, the exponentials and their packing
+// (four prompts of 4000 tokens, causal: 880 TFLOP/s at 128 dims, 765 at 256,
+// 730 at 64, where a large matrix product reaches 1390; with capped scores,
+// three transcendentals each, 740, 710 and 550).  A workgroup owns 128 query
+// rows of one key/value head, a wave 32 of them, and walks the keys they see
+// (or one of `splits` ranges of them) in tiles of 64.  (64 rows per wave: 851
+// for 880, and 655 for 740 capped.)  As many workgroups share a CU as
+// registers allow: their waves are each other's cover.  Tiles arrive in LDS
+// by DMA, one barrier per tile, keys one tile ahead of values.  A wave
 // goes on in halves of 32 keys, three of which are in work at once: the
 // scores of half h + 1 and the output of half h - 1 are on the matrix cores
 // while the exponentials of half h are taken.
@@ -663,9 +672,8 @@ __device__ __forceinline__ float add_pair(uint32_t w, float l) {
 // The products with their operands where the kernel wants them: scores in
 // vector registers, which the exponentials read; output and queries in
 // accumulation registers, which nothing else reads in the common path.  (The
-// compiler would copy scores or output from one file to the other in every
-// half: 3.4 us a tile of 64 keys and 256 rows of 128 dims.)  It does not know
-// when these products finish: what reads their results must come 20 wait
+// compiler by itself copies scores or output from one file to the other in
+// every half.)  It does not know when these products finish: what reads their results must come 20 wait
 // states or more behind the last one (mfma_settle).  NOP: the operand of the
 // vector registers is just computed, which needs two wait states.
 template <bool FIRST, bool NOP>
@@ -707,7 +715,8 @@ struct ProShape {
   // Products of a half: JA steps of the output, the scores' NC, the rest of
   // the output's NO.  Their operand fragments come from LDS in that order,
   // through a ring of registers, read kAhead fragments before their product.
-  // An output step is (block pair, step u, block); e4m3 fragments hold both steps u of a block, or two steps of the scores.
+  // An output step is (block pair, step u, block); e4m3 fragments hold both
+  // steps u of a block, or two steps of the scores.
   static constexpr int NVR = F8 ? NDB : 2 * NDB;  // fragments of values
   static constexpr int NKR = F8 ? NS / 2 : NS;    // fragments of keys
   static constexpr int NO = 2 * NDB, NC = NS, JA = NO / 2;
@@ -1334,6 +1343,10 @@ static PagedPlan paged_plan(const fvx_paged_attn_desc* d) {
   PagedPlan a = {};
   const int64_t G = d->q_heads / d->kv_heads;
   const int64_t most = d->q_start ? d->max_q : 1;
+  // Up to 16 rows are one tile of the few kernel, which would read keys again
+  // for each further one (20 to 64 rows, per sequence 1000 to 4000 keys: 1.2
+  // to 2.7 times the many kernel's time throughout; 16 sequences of 40 rows
+  // of 256 dims: 36 us and 25; one of 20 rows of 64 dims: 27 and 16).
   a.many = most == 0 || most * G > kDecRows;
   // every sequence has most rows: none is left to the few kernel
   a.few = !a.many || most == 0 || d->n_rows != d->n_seqs * most;
@@ -1349,7 +1362,9 @@ static PagedPlan paged_plan(const fvx_paged_attn_desc* d) {
     // With fewer problems than workgroups that run at once their keys are
     // split, no finer than tiles of 64 keys and into 64 ranges at most, whose
     // partials cost as much as they save (one sequence of 4000 keys, 40 rows
-    // of 256 dims: 62 us in 128 ranges).
+    // of 256 dims: 62 us in 128 ranges, 17 in 64).  Fewer ranges than run at
+    // once are slower: 16 sequences of 40 rows of 256 dims 26.5 us, 32 with
+    // half as many; one of 816 tokens of 8 heads 33 and 38.
     const int64_t at_once =
         device_cus() * (d->head_dim == 256 ? ProShape<256, false>::WGS
                                            : (d->head_dim == 128 ? ProShape<128, false>::WGS
@@ -1506,7 +1521,7 @@ extern "C" int fvx_paged_attention(const fvx_paged_attn_desc* d, void* stream) {
   // With a problem or more per workgroup short ones lie behind each other:
   // each counts 128 KiB more, which is what a CU reads while one begins and
   // ends (about 5 us; 64 sequences of 1 to 8192 tokens, 8 heads of 128 dims:
-  // 211 us without, 196 with).
+  // 209 us without, 191 with).
   p.extra = d->n_seqs * d->kv_heads >= plan.n_wg
                 ? (int)((128 << 10) / (2 * d->head_dim * 64)) : 0;
   p.most_rows = plan.most_rows;
