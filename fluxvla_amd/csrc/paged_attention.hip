@@ -1360,18 +1360,24 @@ static PagedPlan paged_plan(const fvx_paged_attn_desc* d) {
     constexpr int64_t bm = ProShape<64, false>::BM;  // of any
     a.problems = (d->n_rows * G / bm + (d->n_seqs < d->n_rows ? d->n_seqs : d->n_rows)) * d->kv_heads;
     // With fewer problems than workgroups that run at once their keys are
-    // split, no finer than tiles of 64 keys and into 64 ranges at most, whose
-    // partials cost as much as they save (one sequence of 4000 keys, 40 rows
-    // of 256 dims: 62 us in 128 ranges, 17 in 64).  Fewer ranges than run at
-    // once are slower: 16 sequences of 40 rows of 256 dims 26.5 us, 32 with
-    // half as many; one of 816 tokens of 8 heads 33 and 38.
+    // split.  Each range costs the merge a partial, and saves the walk of the
+    // others a share of the T tiles of 64 keys that the tables can hold: both
+    // are even at a number of ranges like sqrt(T), 4 sqrt(T) by measurement.
+    // One sequence, 5 tokens of 8 heads of 256 dims (32, 64, 128 ranges):
+    // 4000 keys 18.9, 19.3, 19.1 us; 16000 31.2, 25.3, 24.2; 64000 76.0,
+    // 48.3, 35.6; 16 of 16 heads of 64 dims: 14.0, 15.3, 15.6; 20.0, 18.3,
+    // 22.1; 45.3, 30.2, 27.1.  (Tables may hold more than the lengths use:
+    // 128 at most.)  Fewer ranges than run at once are slower: 16 sequences
+    // of 40 rows of 256 dims 26.8 us, 32.2 with half as many; one of 816
+    // tokens of 8 heads 33.8 and 38.0.
     const int64_t at_once =
         device_cus() * (d->head_dim == 256 ? ProShape<256, false>::WGS
                                            : (d->head_dim == 128 ? ProShape<128, false>::WGS
                                                                  : ProShape<64, false>::WGS));
     const int64_t tiles = (d->max_pages * d->page_size + 63) / 64;
     int64_t s = at_once / a.problems;
-    s = s < 64 ? s : 64;
+    s = s < 128 ? s : 128;
+    while (s > 1 && s * s > 16 * tiles) --s;
     s = s < tiles ? s : tiles;
     a.splits = s < 1 ? 1 : (int)s;
     if (a.splits > 1) {
